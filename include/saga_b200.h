@@ -57,6 +57,7 @@ typedef enum {
 #define SAGA_STATUS_EMPTY_ROW 0x8      /* some row selected nothing (output is NaN) */
 #define SAGA_STATUS_APPEND_RANGE 0x10  /* append_pos_dev held a position outside [0, L): no append */
 #define SAGA_STATUS_PAGE_RANGE 0x20    /* a page table entry outside [0, num_pages): page 0 was read */
+#define SAGA_STATUS_OUT_OF_PAGES 0x40  /* saga_page_tables: a request's new tokens got no pages */
 
 /* Descriptor shared by the attention entry points. Unused fields are ignored.
  * Strides are in elements. */
@@ -245,6 +246,126 @@ SAGA_API int saga_kv_append(int32_t dtype, int32_t B, int32_t Hk, int32_t Hv, in
                    int64_t v_sb, int64_t v_sh, int64_t v_sl, const void* k_new, int64_t kn_sb,
                    int64_t kn_sh, const void* v_new, int64_t vn_sb, int64_t vn_sh,
                    void* stream);
+
+/* ------------------------------------------------------------------------
+ * Serving with a paged cache in 4 bits. No counterpart in the reference, whose
+ * caches are 16-bit tensors of one length for the whole batch.
+ *
+ * The cache. A row (one token, one head) of D values is cut into groups of 64.
+ * With every step in binary32: z = the group's least value rounded down to
+ * bfloat16; s = (greatest - z) * (1/15), at least 2^-40, rounded up to
+ * bfloat16; code = (x - z) * (1/s) rounded to nearest even, within 0..15. The
+ * group stands for s * code + z. A group that holds a NaN or an infinity (or
+ * whose s or z is not finite) stands for NaN.
+ *
+ * A pool holds num_pages pages of page_len positions. A position's slot is
+ * page * page_len + offset. Pages are opaque to callers: [num_pages][H]
+ * [page_len / 32] tiles of 32 positions, each 32 * D/2 bytes of codes followed
+ * by 32 * D/64 pairs (s, z) of bfloat16. A new pool is zero-filled.
+ * ------------------------------------------------------------------------ */
+typedef struct SagaKv4Pool {
+  int32_t Hk, Hv, D;          /* D: 64 or 128 */
+  int32_t page_len;           /* a power of two, at least 32 */
+  int32_t num_pages;
+  void* k; void* v;           /* page tiles, num_pages * H * page_len * (D/2 + D/16) bytes, 16-byte aligned */
+  /* Optional key bounds (both or neither), bfloat16 [num_pages][Hk][D]: the
+   * least and the greatest value that the page's keys stand for, per channel,
+   * rounded outwards. Taken when a page's last slot is written. */
+  void* k_lo; void* k_hi;
+} SagaKv4Pool;
+
+/* Bytes of one page of one head (0 plus an error message for an unsupported
+ * head_dim or page_len). */
+SAGA_API size_t saga_kv4_page_bytes(int32_t D, int32_t page_len);
+
+/* Quantises T rows of keys [T, Hk, D] and values [T, Hv, D] (unit stride along
+ * D, other strides in elements) into the slots of the pool. Slot -1 skips the
+ * row; another slot outside the pool sets SAGA_STATUS_PAGE_RANGE and skips it.
+ * Two rows must not name the same slot. With bounds, a page whose last slot is
+ * among the slots gets its bounds from all its page_len rows. */
+SAGA_API int saga_kv4_write(const SagaKv4Pool* pool, int32_t dtype, int64_t T, const void* k, int64_t k_st,
+                            int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
+                            int32_t* status, void* stream);
+
+/* The inverse: writes what the slots stand for, rounded to dtype, into keys
+ * [T, Hk, D] and values [T, Hv, D]. Slot -1 gives zeros; another slot outside
+ * the pool sets SAGA_STATUS_PAGE_RANGE and gives zeros. */
+SAGA_API int saga_kv4_read(const SagaKv4Pool* pool, int32_t dtype, int64_t T, const int64_t* slots, void* k,
+                           int64_t k_st, int64_t k_sh, void* v, int64_t v_st, int64_t v_sh, int32_t* status,
+                           void* stream);
+
+/* Descriptor of the attention over a 4-bit pool and of the block selection. */
+typedef struct SagaKv4Args {
+  SagaKv4Pool pool;
+  int32_t dtype; /* of q and out */
+  int32_t B, Hq; /* Hq a multiple of Hk and of Hv; heads map as in SagaAttnArgs */
+  const void* q; int64_t q_sb, q_sh; /* [B, Hq, 1, D] */
+  void* out; int64_t o_sb, o_sh;     /* [B, Hq, 1, D] (decode) */
+  /* Logical position p of request b lies in page page_table[b * pt_sb + p / page_len].
+   * An entry outside [0, num_pages) sets SAGA_STATUS_PAGE_RANGE; page 0 is read. */
+  const int32_t* page_table; int64_t pt_sb; int32_t max_pages;
+  const int32_t* lens;   /* [B], on the device: request b attends to positions [starts[b], lens[b]) */
+  const int32_t* starts; /* [B] or NULL (0) */
+  float scaling;
+  /* Selected blocks (pages) per request and key head: int32 [B][Hk][top],
+   * ascending, and how many of them count, int32 [B][Hk]. Read by decode
+   * (NULL = every page), written by select (-1 beyond the count). */
+  int32_t* blocks; int32_t* counts; int32_t top;
+  int32_t keep_first, keep_last; /* select: pages always kept at either end; keep_last >= 1 */
+  void* workspace; size_t workspace_bytes; /* saga_kv4_workspace_bytes; its contents do not matter */
+  int32_t* status;
+} SagaKv4Args;
+
+typedef enum { SAGA_KV4_DECODE = 0, SAGA_KV4_SELECT = 1 } saga_kv4_op;
+
+/* Bytes of workspace of a call (0 plus an error message if the shapes are
+ * invalid). Calls that overlap on the GPU need workspaces of their own. */
+SAGA_API size_t saga_kv4_workspace_bytes(const SagaKv4Args* args, int32_t op);
+
+/* Attention of one query position per request over the 4-bit cache. A request
+ * without positions gets zeros. */
+SAGA_API int saga_kv4_decode(const SagaKv4Args* args, void* stream);
+
+/* Selects `top` pages per request and key head. The score of a complete page is
+ * the greatest, over the key head's queries, of sum_d q_d * (q_d > 0 ? hi_d :
+ * lo_d), in binary32, summed by halves (d with d + D/2, then d + D/4, ...). The
+ * first keep_first and the last keep_last pages of [0, lens[b]) are always
+ * kept; of equal scores the lower page is kept; NaN counts as lowest. Requests
+ * with at most `top` pages keep them all. Needs the pool's bounds. */
+SAGA_API int saga_kv4_select(const SagaKv4Args* args, void* stream);
+
+/* Block tables and slot maps of one step, from the requests' lengths. Request b
+ * holds lens[b] positions and adds new_lens[b]; its tokens are the rows
+ * offsets[b] .. offsets[b + 1] of the step's num_tokens rows. Pages are taken
+ * from the front of a ring of free pages, in order of the requests; a request
+ * whose pages, table row or token rows do not suffice gets nothing: its tokens
+ * get slot -1, its length stays and SAGA_STATUS_OUT_OF_PAGES is set. new_lens[b]
+ * < 0 finishes request b: its pages go to the ring's end and its length becomes
+ * 0. lens_out and free_state_out may be lens and free_state themselves. */
+typedef struct SagaPageTableArgs {
+  int32_t B, page_len, max_pages;
+  int32_t* page_table; int64_t pt_sb;             /* [B, max_pages], entries of new pages are written */
+  const int32_t* lens; const int32_t* new_lens;   /* [B] */
+  int32_t* free_pages; int32_t ring;              /* ring of `ring` entries */
+  const int32_t* free_state;                      /* [2]: index of the first free entry, number of free entries */
+  int64_t num_tokens;
+  int64_t* slots;                                 /* [num_tokens], -1 where there is no token */
+  int32_t* positions;                             /* [num_tokens], 0 where there is no token */
+  int32_t* offsets;                               /* [B + 1] */
+  int32_t* lens_out;                              /* [B] */
+  int32_t* free_state_out;                        /* [2] */
+  void* workspace; size_t workspace_bytes;        /* 16 * B bytes; its contents do not matter */
+  int32_t* status;
+} SagaPageTableArgs;
+
+SAGA_API int saga_page_tables(const SagaPageTableArgs* args, void* stream);
+
+/* The slots of positions [starts[b], lens[b]) (starts NULL = 0) of every
+ * request, packed in order of the requests; offsets int32 [B + 1]. Rows beyond
+ * the last position get -1. */
+SAGA_API int saga_slot_map(int32_t B, int32_t page_len, const int32_t* page_table, int64_t pt_sb, int32_t max_pages,
+                           const int32_t* starts, const int32_t* lens, int64_t num_tokens, int64_t* slots,
+                           int32_t* offsets, int32_t* status, void* stream);
 
 /* Set-up helpers of sequence sharding (no counterpart in the reference).
  * saga_ipc_handle writes the 64-byte cudaIpcMemHandle of the device

@@ -21,6 +21,9 @@ STATUS_OVERFLOW = 0x4
 STATUS_EMPTY_ROW = 0x8
 STATUS_APPEND_RANGE = 0x10
 STATUS_PAGE_RANGE = 0x20
+STATUS_OUT_OF_PAGES = 0x40
+
+SAGA_KV4_DECODE, SAGA_KV4_SELECT = 0, 1
 
 _i32, _i64, _f32, _vp, _sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
@@ -50,6 +53,35 @@ class SagaAttnArgs(ctypes.Structure):
     ]
 
 
+class SagaKv4Pool(ctypes.Structure):
+    """Mirror of ``SagaKv4Pool`` in include/saga_b200.h."""
+    _fields_ = [("Hk", _i32), ("Hv", _i32), ("D", _i32), ("page_len", _i32), ("num_pages", _i32),
+                ("k", _vp), ("v", _vp), ("k_lo", _vp), ("k_hi", _vp)]
+
+
+class SagaKv4Args(ctypes.Structure):
+    """Mirror of ``SagaKv4Args`` in include/saga_b200.h."""
+    _fields_ = [
+        ("pool", SagaKv4Pool), ("dtype", _i32), ("B", _i32), ("Hq", _i32),
+        ("q", _vp), ("q_sb", _i64), ("q_sh", _i64),
+        ("out", _vp), ("o_sb", _i64), ("o_sh", _i64),
+        ("page_table", _vp), ("pt_sb", _i64), ("max_pages", _i32),
+        ("lens", _vp), ("starts", _vp), ("scaling", _f32),
+        ("blocks", _vp), ("counts", _vp), ("top", _i32), ("keep_first", _i32), ("keep_last", _i32),
+        ("workspace", _vp), ("workspace_bytes", _sz), ("status", _vp),
+    ]
+
+
+class SagaPageTableArgs(ctypes.Structure):
+    """Mirror of ``SagaPageTableArgs`` in include/saga_b200.h."""
+    _fields_ = [
+        ("B", _i32), ("page_len", _i32), ("max_pages", _i32), ("page_table", _vp), ("pt_sb", _i64),
+        ("lens", _vp), ("new_lens", _vp), ("free_pages", _vp), ("ring", _i32), ("free_state", _vp),
+        ("num_tokens", _i64), ("slots", _vp), ("positions", _vp), ("offsets", _vp), ("lens_out", _vp),
+        ("free_state_out", _vp), ("workspace", _vp), ("workspace_bytes", _sz), ("status", _vp),
+    ]
+
+
 # (name, restype, argtypes) of every exported function
 SIGNATURES = {
     "saga_workspace_bytes": (_sz, [ctypes.POINTER(SagaAttnArgs), _i32]),
@@ -65,6 +97,16 @@ SIGNATURES = {
                                   _i32, _vp, _i64, _i64, _vp]),
     "saga_kv_append": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
                               _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "saga_kv4_page_bytes": (_sz, [_i32, _i32]),
+    "saga_kv4_write": (_i32, [ctypes.POINTER(SagaKv4Pool), _i32, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                              _vp]),
+    "saga_kv4_read": (_i32, [ctypes.POINTER(SagaKv4Pool), _i32, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                             _vp]),
+    "saga_kv4_workspace_bytes": (_sz, [ctypes.POINTER(SagaKv4Args), _i32]),
+    "saga_kv4_decode": (_i32, [ctypes.POINTER(SagaKv4Args), _vp]),
+    "saga_kv4_select": (_i32, [ctypes.POINTER(SagaKv4Args), _vp]),
+    "saga_page_tables": (_i32, [ctypes.POINTER(SagaPageTableArgs), _vp]),
+    "saga_slot_map": (_i32, [_i32, _i32, _vp, _i64, _i32, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "saga_ipc_handle": (_i32, [_vp, _vp, ctypes.POINTER(_sz)]),
     "saga_ipc_open": (_i32, [_vp, ctypes.POINTER(_vp)]),
     "saga_ipc_close": (_i32, [_vp]),

@@ -131,6 +131,14 @@ int run_attn(const SagaAttnArgs* a, int op, void* stream) {
 namespace saga {
 // Error reporting for entry points defined in other files.
 int abi_fail(int code, const std::string& msg) { return fail(code, msg); }
+void abi_begin() {
+  g_err.clear();
+  g_launched.clear();
+}
+void abi_launched(const char* name) {
+  if (!g_launched.empty()) g_launched += ',';
+  g_launched += name;
+}
 // The full host-side validation of an attention call (no launch).
 int abi_check(const SagaAttnArgs* a, int op) {
   int rc = check_shapes(a);

@@ -1,0 +1,231 @@
+// Block tables and slot maps of a step, built on the GPU from the requests'
+// lengths. The sums over the requests are one CTA's scan; the tokens and the
+// returned pages are then independent of one another.
+#include "kv4.cuh"
+
+namespace saga {
+
+namespace {
+
+constexpr int kScan = 1024;  // threads of the scanning CTA
+
+// Per request, for the token phase (the 16 bytes per request of the workspace).
+struct TableRow {
+  int len;    // positions held before the step; -1: no new tokens are placed
+  int first;  // index in the ring of the request's first new page
+  int back;   // index in the ring of the first page that the request returns; -1: none
+  int held;   // pages held before the step
+};
+
+// Exclusive sums over the CTA's threads of three values; totals in tot.
+__device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], long long (*sm)[33]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long inc[3];
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    long long x = v[j];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    inc[j] = x;
+    if (lane == 31) sm[j][warp] = x;
+  }
+  __syncthreads();
+  if (warp < 3) {
+    const long long own = sm[warp][lane];
+    long long x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncwarp();
+    sm[warp][lane] = x - own;
+    if (lane == 31) sm[warp][32] = x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    tot[j] = sm[j][32];
+    v[j] = sm[j][warp] + inc[j] - v[j];
+  }
+  __syncthreads();
+}
+
+__device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
+  __shared__ long long sm[3][33];
+  const int shift = __ffs(a.page_len) - 1;
+  const long long cover = (long long)a.max_pages << shift;
+  const int head = a.free_state[0];
+  const int count = min(max(a.free_state[1], 0), a.ring);
+  const int h0 = a.ring ? (int)((unsigned)max(head, 0) % (unsigned)a.ring) : 0;
+  long long tok = 0, want = 0, ret = 0, taken = 0;
+  for (int base = 0; base < a.B; base += kScan) {
+    const int b = base + threadIdx.x;
+    const bool in = b < a.B;
+    const int len = in ? max(a.lens[b], 0) : 0;
+    const int raw = in ? a.new_lens[b] : 0;
+    const int add = max(raw, 0);
+    const long long end = (long long)len + add;
+    const int held = (int)(((long long)len + a.page_len - 1) >> shift);
+    long long v[3] = {add, 0, 0}, tot[3];
+    scan3(v, tot, sm);
+    const long long start = tok + v[0];
+    tok += tot[0];
+    const bool fits = end <= cover && start + add <= a.num_tokens;
+    const int need = fits ? (int)(((end + a.page_len - 1) >> shift) - held) : 0;
+    const int back = in && raw < 0 && a.ring ? min(held, a.max_pages) : 0;
+    v[0] = 0;
+    v[1] = need;
+    v[2] = back;
+    scan3(v, tot, sm);
+    const long long upto = want + v[1] + need;
+    const bool granted = fits && (need == 0 || upto <= count);
+    const long long before = ret + v[2];
+    want += tot[1];
+    ret += tot[2];
+    v[0] = granted ? need : 0;
+    v[1] = v[2] = 0;
+    scan3(v, tot, sm);
+    taken += tot[0];
+    if (in) {
+      TableRow r;
+      r.len = granted ? len : -1;
+      r.first = a.ring ? (int)((h0 + upto - need) % a.ring) : 0;
+      r.back = back ? (int)((h0 + (long long)count + before) % a.ring) : -1;
+      r.held = held;
+      rows[b] = r;
+      a.offsets[b + 1] = (int)min(start + add, 0x7fffffffll);
+      a.lens_out[b] = raw < 0 ? 0 : granted ? (int)end : len;
+      if (!granted && add > 0) set_status(a.status, SAGA_STATUS_OUT_OF_PAGES);
+    }
+  }
+  if (threadIdx.x == 0) {
+    a.offsets[0] = 0;
+    a.free_state_out[0] = a.ring ? (int)((h0 + taken) % a.ring) : 0;
+    a.free_state_out[1] = (int)(count - taken + ret);
+  }
+}
+
+// Token `i`: its request by bisection of the offsets, its slot and position;
+// the first token of a new page also writes the page table's entry.
+__device__ __forceinline__ void table_token(const SagaPageTableArgs& a, const TableRow* rows, int64_t i) {
+  int lo = 0, hi = a.B;  // offsets[lo] <= i; hi: first request that begins after i
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.offsets[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  int64_t slot = -1;
+  int pos = 0;
+  if (a.B > 0 && i < a.offsets[a.B]) {
+    const TableRow r = rows[lo];
+    if (r.len >= 0) {
+      pos = r.len + (int)(i - a.offsets[lo]);
+      const int shift = __ffs(a.page_len) - 1;
+      const int p = pos >> shift, off = pos & (a.page_len - 1);
+      int32_t* entry = a.page_table + (int64_t)lo * a.pt_sb + p;
+      int page;
+      if (p < r.held) {
+        page = *entry;
+      } else {
+        page = a.free_pages[((unsigned)r.first + (unsigned)(p - r.held)) % (unsigned)a.ring];
+        if (off == 0) *entry = page;
+      }
+      slot = (int64_t)page * a.page_len + off;
+    }
+  }
+  a.slots[i] = slot;
+  a.positions[i] = pos;
+}
+
+// A warp returns the pages of request b to the ring.
+__device__ __forceinline__ void table_return(const SagaPageTableArgs& a, const TableRow* rows, int b) {
+  const TableRow r = rows[b];
+  if (r.back < 0) return;
+  for (int j = threadIdx.x & 31; j < min(r.held, a.max_pages); j += 32)
+    a.free_pages[((unsigned)r.back + (unsigned)j) % (unsigned)a.ring] = a.page_table[(int64_t)b * a.pt_sb + j];
+}
+
+__global__ void __launch_bounds__(kScan) page_tables_scan_kernel(SagaPageTableArgs a, bool all) {
+  TableRow* rows = reinterpret_cast<TableRow*>(a.workspace);
+  table_scan(a, rows);
+  if (!all) return;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < a.num_tokens; i += kScan) table_token(a, rows, i);
+  for (int b = threadIdx.x >> 5; b < a.B; b += kScan / 32) table_return(a, rows, b);
+}
+
+__global__ void __launch_bounds__(256) page_tables_token_kernel(SagaPageTableArgs a) {
+  const TableRow* rows = reinterpret_cast<const TableRow*>(a.workspace);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < a.num_tokens) table_token(a, rows, i);
+  for (int b = (int)(i >> 5); b < a.B; b += (int)gridDim.x * 8) table_return(a, rows, b);
+}
+
+__global__ void __launch_bounds__(kScan) slot_offsets_kernel(int B, int64_t cover, const int32_t* starts,
+                                                             const int32_t* lens, int32_t* offsets, int* status) {
+  __shared__ long long sm[3][33];
+  long long tok = 0;
+  for (int base = 0; base < B; base += kScan) {
+    const int b = base + threadIdx.x;
+    long long n = 0;
+    if (b < B) {
+      long long end = lens[b];
+      if (end > cover) {
+        set_status(status, SAGA_STATUS_PAGE_RANGE);
+        end = cover;
+      }
+      n = max(end - max(starts ? starts[b] : 0, 0), 0ll);
+    }
+    long long v[3] = {n, 0, 0}, tot[3];
+    scan3(v, tot, sm);
+    if (b < B) offsets[b + 1] = (int)min(tok + v[0] + n, 0x7fffffffll);
+    tok += tot[0];
+  }
+  if (threadIdx.x == 0) offsets[0] = 0;
+}
+
+__global__ void __launch_bounds__(256) slot_map_kernel(int B, int page_len, const int32_t* pt, int64_t pt_sb,
+                                                       const int32_t* starts, int64_t T_, int64_t* slots,
+                                                       const int32_t* offsets) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= T_) return;
+  int64_t slot = -1;
+  if (B > 0 && i < offsets[B]) {
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (offsets[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    const int pos = max(starts ? starts[lo] : 0, 0) + (int)(i - offsets[lo]);
+    const int shift = __ffs(page_len) - 1;
+    slot = (int64_t)pt[(int64_t)lo * pt_sb + (pos >> shift)] * page_len + (pos & (page_len - 1));
+  }
+  slots[i] = slot;
+}
+
+}  // namespace
+
+int launch_page_tables(const SagaPageTableArgs& a, cudaStream_t st) {
+  const bool all = a.num_tokens <= 2048;
+  page_tables_scan_kernel<<<1, kScan, 0, st>>>(a, all);
+  int rc = kv4_launched("page_tables_scan_kernel");
+  if (rc || all) return rc;
+  page_tables_token_kernel<<<(unsigned)((a.num_tokens + 255) / 256), 256, 0, st>>>(a);
+  return kv4_launched("page_tables_token_kernel");
+}
+
+int launch_slot_map(int B, int page_len, const int32_t* pt, int64_t pt_sb, int max_pages, const int32_t* starts,
+                    const int32_t* lens, int64_t T, int64_t* slots, int32_t* offsets, int* status, cudaStream_t st) {
+  slot_offsets_kernel<<<1, kScan, 0, st>>>(B, (int64_t)max_pages * page_len, starts, lens, offsets, status);
+  int rc = kv4_launched("slot_offsets_kernel");
+  if (rc || T == 0) return rc;
+  slot_map_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(B, page_len, pt, pt_sb, starts, T, slots, offsets);
+  return kv4_launched("slot_map_kernel");
+}
+
+}  // namespace saga
