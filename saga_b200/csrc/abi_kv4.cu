@@ -25,6 +25,8 @@ int check_geometry(int32_t D, int32_t page_len) {
 int check_pool(const SagaKv4Pool& p) {
   if (int rc = check_geometry(p.D, p.page_len)) return rc;
   if (p.Hk <= 0 || p.Hv <= 0 || p.num_pages <= 0) return invalid("Hk, Hv and num_pages must be positive");
+  if ((int64_t)p.num_pages * (p.page_len / saga::kKv4Tile) > 0x7fffffffll)
+    return abi_fail(SAGA_ERR_UNSUPPORTED, "the pool has more than 2^31 tiles");
   if (!p.k || !p.v || !aligned(p.k, 16) || !aligned(p.v, 16))
     return invalid("the pool's keys and values must be non-NULL and 16-byte aligned");
   if ((p.k_lo == nullptr) != (p.k_hi == nullptr)) return invalid("k_lo and k_hi go together");
@@ -49,6 +51,8 @@ int check_shapes(const SagaKv4Args* a, int op) {
     return invalid("B >= 0, Hq, Hk, Hv > 0 required");
   if (a->Hq % a->pool.Hk) return invalid("Hq must be a multiple of Hk");
   if (a->Hq % a->pool.Hv) return invalid("Hq must be a multiple of Hv");
+  if ((int64_t)a->B * a->Hq > 0x7fffffffll || (int64_t)a->B * a->pool.Hk > 0x7fffff00ll)
+    return abi_fail(SAGA_ERR_UNSUPPORTED, "too many (request, query head) rows");
   if (a->max_pages <= 0) return invalid("max_pages must be positive");
   if (op == SAGA_KV4_SELECT || a->blocks) {
     if (a->top <= 0) return invalid("top must be positive");
