@@ -14,6 +14,13 @@
 
 namespace saga {
 
+// Waits until the kernels before this one in the stream have finished and their
+// writes can be seen, then lets the next one start its own wait.
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
 template <int D>
 __device__ __forceinline__ int kv4_swizzle(int row) {
   return D == 128 ? (row >> 1) & 3 : (row >> 2) & 1;

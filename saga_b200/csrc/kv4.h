@@ -32,10 +32,28 @@ int launch_page_tables(const SagaPageTableArgs& a, cudaStream_t st);
 int launch_slot_map(int B, int page_len, const int32_t* pt, int64_t pt_sb, int max_pages, const int32_t* starts,
                     const int32_t* lens, int64_t T, int64_t* slots, int32_t* offsets, int* status, cudaStream_t st);
 
-// SAGA_OK, or SAGA_ERR_CUDA with the launch's error.
-inline int kv4_launched(const char* name) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return abi_fail(SAGA_ERR_CUDA, std::string(name) + ": " + cudaGetErrorString(e));
+// Launches a kernel that may start while the one before it in the stream is
+// still running. Every kernel launched so begins with pdl_wait() (kv4.cuh),
+// before it touches memory: what comes before it in the stream has then
+// finished, whether or not it was launched this way.
+template <class... P, class... A>
+int kv4_launch(const char* name, void (*fn)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+               A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return abi_fail(SAGA_ERR_CUDA, std::string(name) + ": " + cudaGetErrorString(e));
+  }
   abi_launched(name);
   return SAGA_OK;
 }

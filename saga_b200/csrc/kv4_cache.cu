@@ -47,6 +47,7 @@ template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256) kv4_write_kernel(const T* __restrict__ k, const T* __restrict__ v, Rows kr,
                                                         Rows vr, int64_t T_, const int64_t* __restrict__ slots,
                                                         int page_len, int num_pages, int* status) {
+  pdl_wait();
   constexpr int NG = D / 64;
   const int l = threadIdx.x & (kLanesPerGroup - 1);
   const int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanesPerGroup;
@@ -111,6 +112,7 @@ template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256) kv4_read_kernel(T* __restrict__ k, T* __restrict__ v, Rows kr, Rows vr,
                                                        int64_t T_, const int64_t* __restrict__ slots, int page_len,
                                                        int num_pages, int* status) {
+  pdl_wait();
   constexpr int NG = D / 64;
   const int l = threadIdx.x & (kLanesPerGroup - 1);
   const int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanesPerGroup;
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t 
                                                          const int64_t* __restrict__ slots) {
   constexpr int W = D / 8, ROWS = 128 / W;
   __shared__ float red[2][ROWS][D];
+  pdl_wait();
   const int w = threadIdx.x % W, rr = threadIdx.x / W;
   for (int64_t t = (int64_t)blockIdx.x * strip; t < min((int64_t)(blockIdx.x + 1) * strip, T_); ++t) {
     const int64_t slot = slots[t];
@@ -234,19 +237,18 @@ int launch_kv4_write(const SagaKv4Pool& p, int dt, int64_t T, const void* k, int
   const int64_t threads = T * (p.Hk + p.Hv) * (p.D / 64) * kLanesPerGroup;
   const int64_t grid = (threads + 255) / 256;
   if (grid > 0x7fffffffll) return abi_fail(SAGA_ERR_UNSUPPORTED, "too many rows for one call");
+  int rc = SAGA_OK;
   dispatch(dt, p.D, vec, [&](auto* t, auto d, auto a) {
     using E = std::remove_pointer_t<decltype(t)>;
-    kv4_write_kernel<E, d.value, a.value><<<(unsigned)grid, 256, 0, st>>>(
-        reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v), kr, vr, T, slots, p.page_len, p.num_pages,
-        status);
+    rc = kv4_launch("kv4_write_kernel", kv4_write_kernel<E, d.value, a.value>, dim3((unsigned)grid), 256, 0, st,
+                    reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v), kr, vr, T, slots, p.page_len,
+                    p.num_pages, status);
   });
-  int rc = kv4_launched("kv4_write_kernel");
   if (rc || !p.k_lo) return rc;
   const int strip = T <= 4096 ? 1 : 32;
   const unsigned nb = (unsigned)((T + strip - 1) / strip);
-  if (p.D == 128) kv4_bounds_kernel<128><<<nb, 128, 0, st>>>(p, T, strip, slots);
-  else kv4_bounds_kernel<64><<<nb, 128, 0, st>>>(p, T, strip, slots);
-  return kv4_launched("kv4_bounds_kernel");
+  return kv4_launch("kv4_bounds_kernel", p.D == 128 ? kv4_bounds_kernel<128> : kv4_bounds_kernel<64>, dim3(nb), 128, 0,
+                    st, p, T, strip, slots);
 }
 
 int launch_kv4_read(const SagaKv4Pool& p, int dt, int64_t T, const int64_t* slots, void* k, int64_t k_st,
@@ -258,12 +260,14 @@ int launch_kv4_read(const SagaKv4Pool& p, int dt, int64_t T, const int64_t* slot
   const int64_t threads = T * (p.Hk + p.Hv) * (p.D / 64) * kLanesPerGroup;
   const int64_t grid = (threads + 255) / 256;
   if (grid > 0x7fffffffll) return abi_fail(SAGA_ERR_UNSUPPORTED, "too many rows for one call");
+  int rc = SAGA_OK;
   dispatch(dt, p.D, vec, [&](auto* t, auto d, auto a) {
     using E = std::remove_pointer_t<decltype(t)>;
-    kv4_read_kernel<E, d.value, a.value><<<(unsigned)grid, 256, 0, st>>>(
-        reinterpret_cast<E*>(k), reinterpret_cast<E*>(v), kr, vr, T, slots, p.page_len, p.num_pages, status);
+    rc = kv4_launch("kv4_read_kernel", kv4_read_kernel<E, d.value, a.value>, dim3((unsigned)grid), 256, 0, st,
+                    reinterpret_cast<E*>(k), reinterpret_cast<E*>(v), kr, vr, T, slots, p.page_len, p.num_pages,
+                    status);
   });
-  return kv4_launched("kv4_read_kernel");
+  return rc;
 }
 
 }  // namespace saga

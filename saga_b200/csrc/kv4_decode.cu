@@ -37,7 +37,7 @@ constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kMaxSlots = 16;       // query heads of an item
 constexpr int kMaxRing = 4;         // stages of a warp's ring
-constexpr int kMinTiles = kDecWarps;  // tiles of a CTA's run: at least one per warp
+constexpr int kMinTiles = 4;        // tiles of a CTA's run, at least: one warp per scheduler
 constexpr int kRingBytes = 216 * 1024;  // of all warps; static shared memory has the rest
 constexpr float kHead = 12.f;     // log2 of the greatest weight where the stabiliser was last set
 constexpr float kLow = 2048.f;    // SPLIT: the second term of a weight is held this much greater
@@ -72,7 +72,6 @@ struct DecodePlan4 {
   int tpp_shift;   // log2 of the tiles per page
   float* part_o;   // [grid][2][slots][D] numerators of cut items
   float* part_ml;  // [grid][2][slots][2] their maxima and sums
-  long long* trace;
   long long* prefix;  // [rows + 1] tiles before a (request, key head) row
 };
 
@@ -188,11 +187,6 @@ __device__ __forceinline__ long long tiles_per_cta(long long total, int grid) {
   return max((total + grid - 1) / grid, (long long)kMinTiles);
 }
 
-#ifdef KV4_TRACE
-#define KV4_STAMP(i) { if (blockIdx.x == 0 && threadIdx.x == 0) { long long now = clock64(); trc[i] += now - last; last = now; } }
-#else
-#define KV4_STAMP(i)
-#endif
 // D: head_dim; NT: tiles of eight slots; SPLIT: queries and weights as two fp16
 // terms each (fp32 tensors, 22 significant bits).
 template <int D, int NT, bool SPLIT>
@@ -214,9 +208,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   __shared__ float q_unit[kMaxSlots], q_sum[kMaxSlots][2];
   __shared__ float sm_m[kDecWarps][kMaxSlots], sm_l[kDecWarps][kMaxSlots], sm_f[kDecWarps][kMaxSlots];
 
-#ifdef KV4_TRACE
-  long long trc[16] = {}, last = clock64();
-#endif
   const SagaKv4Args& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r8 = lane >> 2, c4 = lane & 3;
@@ -229,7 +220,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     mbar_fence_init();
   }
 
-  KV4_STAMP(0);
+  pdl_wait();
   // ---- this CTA's run of tiles: [run, run_end), and the row it begins in
   long long total = 0;
   if (rows > kDecThreads) {
@@ -280,8 +271,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     __syncthreads();
     if (!writes_prefix && (run >= run_end || base > run)) break;
   }
-  KV4_STAMP(1);
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (run >= run_end) return;
   int row = sh_row;
   long long row_base = sh_row_base;
@@ -364,45 +353,41 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     // positions of the tiles being consumed: the batch that `issue` holds may be one ahead
     int cp0 = ps0, cp1 = ps1;
 
-    const int ahead = min(p.stages - 1, mine);
-    for (int k = 0; k < ahead; ++k) issue(k);
-
-  KV4_STAMP(2);
     // ---- slots of the item's query heads
     if (kh != have_kh || sg != have_sg) {
-      if (threadIdx.x == 0) {
+      if (warp == 0) {
         // a value head's slots stay inside one tile of eight where that fits, since
         // its codes are multiplied with every tile that has one of its slots
-        uint32_t on = 0;
+        int head = -1, vh = -1;
         for (int pass = 0; pass < 2; ++pass) {
           int at = 0, h = grp.h0;
-          on = 0;
-          for (int i = 0; i < SLOTS; ++i) {
-            slot_head[i] = -1;
-            slot_vh[i] = -1;
-          }
+          head = vh = -1;
           for (int v = 0; h < grp.h0 + grp.n; ++v) {
             const int n = min((vh0 + v + 1) * Gv, grp.h0 + grp.n) - h;
             if (pass == 0 && (at & 7) && (at & 7) + min(n, 8) > 8) at = (at + 7) & ~7;
             if (at + n > SLOTS) break;
-            for (int i = 0; i < n; ++i) {
-              slot_head[at + i] = h + i;
-              slot_vh[at + i] = v;
-              on |= 1u << (2 * v + (at + i) / 8);
+            if (lane >= at && lane < at + n) {
+              head = h + lane - at;
+              vh = v;
             }
             at += n;
             h += n;
           }
           if (h >= grp.h0 + grp.n) break;
         }
-        sh_on = on;  // bits 2j, 2j + 1: slot tiles that hold slots of value head j
+        if (lane < kMaxSlots) {
+          slot_head[lane] = head;
+          slot_vh[lane] = vh;
+        }
+        // bits 2j, 2j + 1: slot tiles that hold slots of value head j
+        const uint32_t on = __reduce_or_sync(0xffffffffu, vh < 0 ? 0u : 1u << (2 * vh + lane / 8));
+        if (lane == 0) sh_on = on;
       }
       have_kh = kh;
       have_sg = sg;
       __syncthreads();
     }
 
-  KV4_STAMP(3);
     // ---- queries, scaled by a power of two that brings the greatest |q| of a head into [2^14, 2^15).
     // Order within eight channels: (0, 4) (1, 5) (2, 6) (3, 7), the pairs in which codes leave a word;
     // odd channels' codes are read 16 times too great.
@@ -425,6 +410,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
           for (int i = 0; i < QC; ++i) v[i] = reinterpret_cast<const float*>(a.q)[at + i];
         }
       }
+      // the first copies leave while the queries arrive
+      const int ahead = min(p.stages - 1, mine);
+      for (int k = 0; k < ahead; ++k) issue(k);
 #pragma unroll
       for (int i = 0; i < QC; ++i) amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll
@@ -456,7 +444,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       if (i0 == 0) q_unit[s] = a.scaling * 1.4426950408889634f * down;  // scores in powers of two
     }
     __syncthreads();
-  KV4_STAMP(4);
     f32x2 fh[NT], Qz[NT][NG];    // each value twice
     int vhl[NT];
 #pragma unroll
@@ -484,9 +471,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     }
 
     for (int k = 0; k < mine; ++k) {
-      KV4_STAMP(11);
       if (k + p.stages - 1 < mine) issue(k + p.stages - 1);
-      KV4_STAMP(12);
       if ((k & 31) == 0 && k > 0) {
         cp0 = cp1;
         cp1 = ps1;  // `issue` has moved on to the batch after this one, if there is one
@@ -503,7 +488,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         alive = false;
         break;
       }
-  KV4_STAMP(5);
       const uint32_t ks = ring_s + st_c * stage_bytes;
       uint8_t* kt = ring + st_c * stage_bytes;
       if (++st_c == p.stages) {
@@ -604,7 +588,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         }
       }
 
-  KV4_STAMP(6);
       // ---- stabiliser, raised only when needed: weights p * s of at most 2^15 are left as they are.
       // A new one puts a bound of the greatest weight at 2^kHead, so that weights far below it are still
       // normal in fp16 (11 significant bits down to 2^-14). The bound joins the greatest score of a lane's
@@ -684,7 +667,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         }
       }
 
-  KV4_STAMP(7);
       // ---- output. The tensor cores' sums are not rounded to nearest, so 32 positions are summed there
       // and the running sum is added outside; and the codes are taken about their middle (7.5), since
       // what they have in common grows with the positions, and with it the error, faster than the result.
@@ -747,7 +729,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
           }
         }
       }
-  KV4_STAMP(8);
       __syncwarp();  // every lane has read the stage before its next copy is issued
     }
 
@@ -795,7 +776,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       }
     }
     __syncthreads();
-  KV4_STAMP(9);
     const int busy = min(t1 - t0, kDecWarps);  // warps that had tiles
     if (threadIdx.x < kDecWarps * SLOTS) {
       const int w = threadIdx.x / SLOTS, s = threadIdx.x % SLOTS;
@@ -844,14 +824,10 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         }
       }
     }
-  KV4_STAMP(10);
     fence_proxy_async_smem();  // the ring is written by bulk copies again
     __syncthreads();
     run = item_base + t1;
   }
-#ifdef KV4_TRACE
-  if (blockIdx.x == 0 && threadIdx.x == 0) for (int i = 0; i < 16; ++i) p.trace[i] = trc[i];
-#endif
 }
 
 // Joins the partial results of items that CTA borders cut, and writes the zeros
@@ -873,8 +849,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_combine_kernel(const DecodeP
   int sg = 0;
   SlotGroup grp = slot_group(kh, 0, G, Gv, slots, p.vheads);
   while (h >= grp.h0 + grp.n) grp = slot_group(kh, ++sg, G, Gv, slots, p.vheads);
+  pdl_wait();
   if (threadIdx.x == 0 && a.lens[b] > a.max_pages * a.pool.page_len) set_status(a.status, SAGA_STATUS_PAGE_RANGE);
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const long long total = p.prefix[a.B * a.pool.Hk], first = p.prefix[row];
   const long long tiles = (p.prefix[row + 1] - first) / p.groups;
   const int64_t at = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
@@ -972,7 +948,7 @@ DecodeSizes decode_sizes(const SagaKv4Args& a) {
   const size_t rows = (size_t)a.B * a.pool.Hk;
   z.off_o = ((rows + 1) * sizeof(long long) + 255) / 256 * 256;
   z.off_ml = z.off_o + (size_t)z.grid * 2 * z.slots * D * sizeof(float);
-  z.total = z.off_ml + (size_t)z.grid * 2 * z.slots * 2 * sizeof(float) + 256;
+  z.total = z.off_ml + (size_t)z.grid * 2 * z.slots * 2 * sizeof(float);
   return z;
 }
 
@@ -980,23 +956,20 @@ template <int D, int NT, bool SPLIT>
 int launch(const DecodePlan4& p, const DecodeSizes& z, cudaStream_t st) {
   auto* fn = kv4_decode_kernel<D, NT, SPLIT>;
   const int smem = z.ring_bytes * kDecWarps;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return abi_fail(SAGA_ERR_CUDA, std::string("kv4_decode_kernel: ") + cudaGetErrorString(e));
-  fn<<<z.grid, kDecThreads, smem, st>>>(p);
-  if (int rc = kv4_launched("kv4_decode_kernel")) return rc;
-  // the join may start while the last CTAs of the main kernel still run
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(p.a.B * p.a.Hq));
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = st;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, p, z.grid, z.slots);
-  if (e != cudaSuccess) return abi_fail(SAGA_ERR_CUDA, std::string("kv4_combine_kernel: ") + cudaGetErrorString(e));
-  return kv4_launched("kv4_combine_kernel");
+  // the limit is an attribute of the function on a device; it only rises
+  static thread_local int dev_of = -1, raised = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e;
+  if (dev != dev_of || smem > raised) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (e != cudaSuccess) return abi_fail(SAGA_ERR_CUDA, std::string("kv4_decode_kernel: ") + cudaGetErrorString(e));
+    dev_of = dev;
+    raised = kRingBytes;
+  }
+  if (int rc = kv4_launch("kv4_decode_kernel", fn, dim3(z.grid), kDecThreads, smem, st, p)) return rc;
+  return kv4_launch("kv4_combine_kernel", kv4_combine_kernel<D>, dim3((unsigned)(p.a.B * p.a.Hq)), kJoinThreads, 0, st,
+                    p, z.grid, z.slots);
 }
 
 }  // namespace
@@ -1017,7 +990,6 @@ int launch_kv4_decode(const SagaKv4Args& a, cudaStream_t st) {
   p.prefix = reinterpret_cast<long long*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + z.off_o);
   p.part_ml = reinterpret_cast<float*>(ws + z.off_ml);
-  p.trace = reinterpret_cast<long long*>(ws + z.total - 256);
   if (a.dtype == SAGA_FP32) return a.pool.D == 128 ? launch<128, 1, true>(p, z, st) : launch<64, 1, true>(p, z, st);
   if (z.nt == 1) return a.pool.D == 128 ? launch<128, 1, false>(p, z, st) : launch<64, 1, false>(p, z, st);
   return a.pool.D == 128 ? launch<128, 2, false>(p, z, st) : launch<64, 2, false>(p, z, st);

@@ -150,6 +150,7 @@ __device__ __forceinline__ void table_return(const SagaPageTableArgs& a, const T
 }
 
 __global__ void __launch_bounds__(kScan) page_tables_scan_kernel(SagaPageTableArgs a, bool all) {
+  pdl_wait();
   TableRow* rows = reinterpret_cast<TableRow*>(a.workspace);
   table_scan(a, rows);
   if (!all) return;
@@ -159,6 +160,7 @@ __global__ void __launch_bounds__(kScan) page_tables_scan_kernel(SagaPageTableAr
 }
 
 __global__ void __launch_bounds__(256) page_tables_token_kernel(SagaPageTableArgs a) {
+  pdl_wait();
   const TableRow* rows = reinterpret_cast<const TableRow*>(a.workspace);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < a.num_tokens) table_token(a, rows, i);
@@ -168,6 +170,7 @@ __global__ void __launch_bounds__(256) page_tables_token_kernel(SagaPageTableArg
 __global__ void __launch_bounds__(kScan) slot_offsets_kernel(int B, int64_t cover, const int32_t* starts,
                                                              const int32_t* lens, int32_t* offsets, int* status) {
   __shared__ long long sm[3][33];
+  pdl_wait();
   long long tok = 0;
   for (int base = 0; base < B; base += kScan) {
     const int b = base + threadIdx.x;
@@ -191,6 +194,7 @@ __global__ void __launch_bounds__(kScan) slot_offsets_kernel(int B, int64_t cove
 __global__ void __launch_bounds__(256) slot_map_kernel(int B, int page_len, const int32_t* pt, int64_t pt_sb,
                                                        const int32_t* starts, int64_t T_, int64_t* slots,
                                                        const int32_t* offsets) {
+  pdl_wait();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= T_) return;
   int64_t slot = -1;
@@ -212,20 +216,19 @@ __global__ void __launch_bounds__(256) slot_map_kernel(int B, int page_len, cons
 
 int launch_page_tables(const SagaPageTableArgs& a, cudaStream_t st) {
   const bool all = a.num_tokens <= 2048;
-  page_tables_scan_kernel<<<1, kScan, 0, st>>>(a, all);
-  int rc = kv4_launched("page_tables_scan_kernel");
+  int rc = kv4_launch("page_tables_scan_kernel", page_tables_scan_kernel, dim3(1), kScan, 0, st, a, all);
   if (rc || all) return rc;
-  page_tables_token_kernel<<<(unsigned)((a.num_tokens + 255) / 256), 256, 0, st>>>(a);
-  return kv4_launched("page_tables_token_kernel");
+  return kv4_launch("page_tables_token_kernel", page_tables_token_kernel,
+                    dim3((unsigned)((a.num_tokens + 255) / 256)), 256, 0, st, a);
 }
 
 int launch_slot_map(int B, int page_len, const int32_t* pt, int64_t pt_sb, int max_pages, const int32_t* starts,
                     const int32_t* lens, int64_t T, int64_t* slots, int32_t* offsets, int* status, cudaStream_t st) {
-  slot_offsets_kernel<<<1, kScan, 0, st>>>(B, (int64_t)max_pages * page_len, starts, lens, offsets, status);
-  int rc = kv4_launched("slot_offsets_kernel");
+  int rc = kv4_launch("slot_offsets_kernel", slot_offsets_kernel, dim3(1), kScan, 0, st, B,
+                      (int64_t)max_pages * page_len, starts, lens, offsets, status);
   if (rc || T == 0) return rc;
-  slot_map_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(B, page_len, pt, pt_sb, starts, T, slots, offsets);
-  return kv4_launched("slot_map_kernel");
+  return kv4_launch("slot_map_kernel", slot_map_kernel, dim3((unsigned)((T + 255) / 256)), 256, 0, st, B, page_len, pt,
+                    pt_sb, starts, T, slots, offsets);
 }
 
 }  // namespace saga

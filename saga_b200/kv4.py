@@ -19,26 +19,75 @@ batch (speedup.py:119-139).
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib as L
-from .ops import _dt, _require_cuda, _stream, status_tensor
+from .ops import _DT, _STATUS, status_tensor
 
 GROUP = 64  # values that share a scale
 _SCRATCH: dict = {}
+_I32, _I64 = torch.int32, torch.int64
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _scratch(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Workspace of the calling stream on ``device``. The kernels do not care
-    what it holds. Smaller ones are kept, since a CUDA graph may refer to them."""
-    have = _SCRATCH.setdefault((device.index, _stream(device)), [])
-    if not have or have[-1].numel() < nbytes:
-        grown = max(nbytes, 2 * have[-1].numel() if have else 0)
-        have.append(torch.empty(grown, dtype=torch.uint8, device=device))
-    return have[-1]
+def _scratch(index: int, stream: int, nbytes: int) -> int:
+    """Address of ``nbytes`` of workspace for calls on this stream. The kernels
+    do not care what it holds. Smaller ones are kept, since a CUDA graph may
+    refer to them."""
+    have = _SCRATCH.get((index, stream))
+    if have is None or have[-1].numel() < nbytes:
+        grown = torch.empty(max(nbytes, 2 * have[-1].numel() if have else 1 << 20), dtype=torch.uint8,
+                            device=torch.device("cuda", index))
+        have = _SCRATCH.setdefault((index, stream), [])
+        have.append(grown)
+    return have[-1].data_ptr()
+
+
+def _status(index: int) -> int:
+    t = _STATUS.get(index)
+    return (status_tensor(torch.device("cuda", index)) if t is None else t).data_ptr()
+
+
+class _on_device:
+    """Makes a device current for a C call, where it is not."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.before)
+
+
+def _bad_cuda():
+    raise ValueError("saga_b200 ops take CUDA tensors (there is no CPU path)")
+
+
+def _bad(name: str, t, index: int, dtype, shape):
+    """The error that says what is wrong with an integer argument."""
+    if not t.is_cuda:
+        _bad_cuda()
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {list(shape)}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def _ints(name: str, t, index: int, dtype, shape) -> int:
+    """Address of a contiguous integer tensor of this device, type and shape."""
+    if not (t.dtype is dtype and t.get_device() == index and t.shape == shape and t.is_contiguous()):
+        _bad(name, t, index, dtype, shape)
+    return t.data_ptr()
 
 
 class Kv4Pool:
@@ -68,8 +117,14 @@ class Kv4Pool:
         if bounds:
             self.k_lo, self.k_hi = (torch.zeros((num_pages, key_heads, head_dim), dtype=torch.bfloat16,
                                                 device=self.device) for _ in range(2))
+        self._index = self.device.index
+        self._desc = self.descriptor()
+        self._ref = ctypes.byref(self._desc)
+        self._status = status_tensor(self.device).data_ptr()
+        self._sizes: dict = {}  # workspace bytes per op and shapes
 
     def descriptor(self) -> L.SagaKv4Pool:
+        """The C descriptor of the pool's tensors."""
         p = L.SagaKv4Pool()
         p.Hk, p.Hv, p.D = self.key_heads, self.value_heads, self.head_dim
         p.page_len, p.num_pages = self.page_len, self.num_pages
@@ -82,35 +137,28 @@ class Kv4Pool:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_lo, self.k_hi) if t is not None)
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-
-
-def _int_tensor(name, t, dtype, shape=None, contiguous=True):
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {list(shape)}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t
-
-
-def _rows(pool: Kv4Pool, k, v, slots):
-    _require_cuda(k, v, slots)
-    _same_device(pool.device, k=k, v=v, slots=slots)
+def _rows(pool: Kv4Pool, k, v, slots) -> int:
     T = slots.numel()
-    _int_tensor("slots", slots, torch.int64, (T,))
-    if k.dtype != v.dtype:
-        raise TypeError("k and v must share a dtype")
+    _ints("slots", slots, pool._index, _I64, (T,))
     for name, t, heads in (("k", k, pool.key_heads), ("v", v, pool.value_heads)):
-        if tuple(t.shape) != (T, heads, pool.head_dim):
+        if t.get_device() != pool._index:
+            if not t.is_cuda:
+                _bad_cuda()
+            raise ValueError(f"{name} is on {t.device}, not on {pool.device}")
+        if t.shape != (T, heads, pool.head_dim):
             raise ValueError(f"{name} must be [{T}, {heads}, {pool.head_dim}]")
-        if t.numel() and t.stride(2) != 1:
+        if t.stride(2) != 1 and t.numel():
             raise ValueError(f"{name} needs a unit stride along head_dim")
+    if k.dtype is not v.dtype:
+        raise TypeError("k and v must share a dtype")
     return T
+
+
+def _dtype_code(dtype) -> int:
+    code = _DT.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype} (bf16, fp16 or fp32)")
+    return code
 
 
 def kv4_write(pool: Kv4Pool, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -119,10 +167,12 @@ def kv4_write(pool: Kv4Pool, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
     ``STATUS_PAGE_RANGE`` and skips the row. In a pool with bounds, a page whose
     last slot is written gets its key bounds. Two rows must not name one slot."""
     T = _rows(pool, k, v, slots)
-    with torch.cuda.device(pool.device):
-        L.check(L.lib.saga_kv4_write(ctypes.byref(pool.descriptor()), _dt(k), T, k.data_ptr(), k.stride(0),
-                                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(),
-                                     status_tensor(pool.device).data_ptr(), _stream(pool.device)), "saga_kv4_write")
+    ks, vs = k.stride(), v.stride()
+    with _on_device(pool._index):
+        rc = L.lib.saga_kv4_write(pool._ref, _dtype_code(k.dtype), T, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+                                  vs[1], slots.data_ptr(), pool._status, _raw_stream(pool._index))
+    if rc:
+        L.check(rc, "saga_kv4_write")
 
 
 def kv4_read(pool: Kv4Pool, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
@@ -131,53 +181,79 @@ def kv4_read(pool: Kv4Pool, slots: torch.Tensor, dtype: torch.dtype = torch.bflo
     to ``dtype``; zeros for slot -1 (and, with ``STATUS_PAGE_RANGE``, for a slot
     outside the pool). E.g. the history that a prompt chunk attends to."""
     T = slots.numel()
-    k = torch.empty((T, pool.key_heads, pool.head_dim), dtype=dtype, device=pool.device)
-    v = torch.empty((T, pool.value_heads, pool.head_dim), dtype=dtype, device=pool.device)
-    _rows(pool, k, v, slots)
-    with torch.cuda.device(pool.device):
-        L.check(L.lib.saga_kv4_read(ctypes.byref(pool.descriptor()), _dt(k), T, slots.data_ptr(), k.data_ptr(),
-                                    k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                    status_tensor(pool.device).data_ptr(), _stream(pool.device)), "saga_kv4_read")
+    code = _dtype_code(dtype)
+    at = _ints("slots", slots, pool._index, _I64, (T,))
+    D = pool.head_dim
+    k = torch.empty((T, pool.key_heads, D), dtype=dtype, device=pool.device)
+    v = torch.empty((T, pool.value_heads, D), dtype=dtype, device=pool.device)
+    with _on_device(pool._index):
+        rc = L.lib.saga_kv4_read(pool._ref, code, T, at, k.data_ptr(), pool.key_heads * D, D, v.data_ptr(),
+                                 pool.value_heads * D, D, pool._status, _raw_stream(pool._index))
+    if rc:
+        L.check(rc, "saga_kv4_read")
     return k, v
 
 
-def _table(name, t, B):
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be {torch.int32}")
-    if t.dim() != 2 or t.shape[0] < B or (t.numel() and t.stride(1) != 1):
-        raise ValueError(f"{name} must be an int32 [B, max_pages] tensor with unit column stride")
+def _table(t, index: int, B: int) -> int:
+    if t.dtype is not _I32:
+        raise TypeError(f"page_table must be {_I32}")
+    if not t.is_cuda:
+        _bad_cuda()
+    if t.get_device() != index:
+        raise ValueError(f"page_table is on {t.device}, not on cuda:{index}")
+    if t.dim() != 2 or t.shape[0] < B or (t.stride(1) != 1 and t.numel()):
+        raise ValueError("page_table must be an int32 [B, max_pages] tensor with unit column stride")
+    return t.data_ptr()
 
 
-def _kv4_args(q, pool, page_table, lens):
-    _require_cuda(q, page_table, lens)
-    if q.dim() != 4 or q.shape[2] != 1:
+def _kv4_args(q, pool: Kv4Pool, page_table, lens) -> L.SagaKv4Args:
+    index = pool._index
+    if q.get_device() != index:
+        if not q.is_cuda:
+            _bad_cuda()
+        raise ValueError(f"query is on {q.device}, not on {pool.device}")
+    shape = q.shape
+    if len(shape) != 4 or shape[2] != 1:
         raise ValueError("query must be [B, Hq, 1, D]")
-    B, Hq, _, D = q.shape
-    if D != pool.head_dim:
-        raise ValueError(f"query has head_dim {D}, the pool {pool.head_dim}")
-    if q.numel() and q.stride(3) != 1:
+    if shape[3] != pool.head_dim:
+        raise ValueError(f"query has head_dim {shape[3]}, the pool {pool.head_dim}")
+    qs = q.stride()
+    if qs[3] != 1 and q.numel():
         raise ValueError("query needs a unit stride along head_dim")
-    _same_device(pool.device, query=q, page_table=page_table, lens=lens)
-    _table("page_table", page_table, B)
-    _int_tensor("lens", lens, torch.int32, (B,))
+    B = shape[0]
     a = L.SagaKv4Args()
-    a.pool = pool.descriptor()
-    a.dtype, a.B, a.Hq = _dt(q), B, Hq
-    a.q, a.q_sb, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
-    a.page_table, a.pt_sb, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-    a.lens = lens.data_ptr()
-    a.status = status_tensor(pool.device).data_ptr()
+    a.pool = pool._desc
+    a.dtype = _dtype_code(q.dtype)
+    a.B = B
+    a.Hq = shape[1]
+    a.q = q.data_ptr()
+    a.q_sb = qs[0]
+    a.q_sh = qs[1]
+    a.page_table = _table(page_table, index, B)
+    a.pt_sb = page_table.stride(0)
+    a.max_pages = page_table.shape[1]
+    a.lens = _ints("lens", lens, index, _I32, (B,))
+    a.status = pool._status
     return a
 
 
-def _kv4_run(fn_name, a, op, device):
-    with torch.cuda.device(device):
-        nbytes = L.lib.saga_kv4_workspace_bytes(ctypes.byref(a), op)
-        if nbytes == 0:
-            raise L.SagaError(L.SAGA_ERR_INVALID, "saga_kv4_workspace_bytes")
-        ws = _scratch(device, nbytes)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        L.check(getattr(L.lib, fn_name)(ctypes.byref(a), _stream(device)), fn_name)
+def _kv4_run(fn, name: str, a: L.SagaKv4Args, op: int, pool: Kv4Pool) -> None:
+    index = pool._index
+    with _on_device(index):
+        ref = ctypes.byref(a)
+        key = (op, a.dtype, a.B, a.Hq, a.max_pages, a.top)
+        nbytes = pool._sizes.get(key)
+        if nbytes is None:
+            nbytes = L.lib.saga_kv4_workspace_bytes(ref, op)
+            if nbytes == 0:
+                raise L.SagaError(L.SAGA_ERR_INVALID, "saga_kv4_workspace_bytes")
+            pool._sizes[key] = nbytes
+        stream = _raw_stream(index)
+        a.workspace = _scratch(index, stream, nbytes)
+        a.workspace_bytes = nbytes
+        rc = fn(ref, stream)
+    if rc:
+        L.check(rc, name)
 
 
 def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, lens: torch.Tensor,
@@ -192,26 +268,26 @@ def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     to those pages alone. ``scaling`` defaults to 1/sqrt(D).
     """
     a = _kv4_args(query, pool, page_table, lens)
-    a.scaling = float(1.0 / math.sqrt(a.pool.D) if scaling is None else scaling)
+    B, Hq, D = a.B, a.Hq, pool.head_dim
+    a.scaling = D ** -0.5 if scaling is None else float(scaling)
     if starts is not None:
-        _require_cuda(starts)
-        _same_device(pool.device, starts=starts)
-        a.starts = _int_tensor("starts", starts, torch.int32, (a.B,)).data_ptr()
-    if (blocks is None) != (counts is None):
-        raise ValueError("blocks and counts go together")
-    if blocks is not None:
-        _require_cuda(blocks, counts)
-        _same_device(pool.device, blocks=blocks, counts=counts)
+        a.starts = _ints("starts", starts, pool._index, _I32, (B,))
+    if blocks is not None or counts is not None:
+        if blocks is None or counts is None:
+            raise ValueError("blocks and counts go together")
         if blocks.dim() != 3:
             raise ValueError("blocks must be [B, Hk, top]")
-        a.top = blocks.shape[2]
-        a.blocks = _int_tensor("blocks", blocks, torch.int32, (a.B, pool.key_heads, a.top)).data_ptr()
-        a.counts = _int_tensor("counts", counts, torch.int32, (a.B, pool.key_heads)).data_ptr()
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    if a.B == 0:
+        top = blocks.shape[2]
+        a.top = top
+        a.blocks = _ints("blocks", blocks, pool._index, _I32, (B, pool.key_heads, top))
+        a.counts = _ints("counts", counts, pool._index, _I32, (B, pool.key_heads))
+    out = torch.empty((B, Hq, 1, D), dtype=query.dtype, device=pool.device)
+    if B == 0:
         return out
-    a.out, a.o_sb, a.o_sh = out.data_ptr(), out.stride(0), out.stride(1)
-    _kv4_run("saga_kv4_decode", a, L.SAGA_KV4_DECODE, pool.device)
+    a.out = out.data_ptr()
+    a.o_sb = Hq * D
+    a.o_sh = D
+    _kv4_run(L.lib.saga_kv4_decode, "saga_kv4_decode", a, L.SAGA_KV4_DECODE, pool)
     return out
 
 
@@ -228,15 +304,16 @@ def kv4_select(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     a = _kv4_args(query, pool, page_table, lens)
     if pool.k_lo is None:
         raise ValueError("kv4_select needs a pool with bounds=True")
-    a.top, a.keep_first, a.keep_last = int(top), int(keep_first), int(keep_last)
-    if a.top <= 0:
+    top = int(top)
+    if top <= 0:
         raise ValueError("top must be positive")
-    blocks = torch.empty((a.B, pool.key_heads, a.top), dtype=torch.int32, device=pool.device)
-    counts = torch.empty((a.B, pool.key_heads), dtype=torch.int32, device=pool.device)
+    a.top, a.keep_first, a.keep_last = top, int(keep_first), int(keep_last)
+    blocks = torch.empty((a.B, pool.key_heads, top), dtype=_I32, device=pool.device)
+    counts = torch.empty((a.B, pool.key_heads), dtype=_I32, device=pool.device)
     if a.B == 0:
         return blocks, counts
     a.blocks, a.counts = blocks.data_ptr(), counts.data_ptr()
-    _kv4_run("saga_kv4_select", a, L.SAGA_KV4_SELECT, pool.device)
+    _kv4_run(L.lib.saga_kv4_select, "saga_kv4_select", a, L.SAGA_KV4_SELECT, pool)
     return blocks, counts
 
 
@@ -267,37 +344,44 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     ``lens_out`` and ``free_state_out`` may be ``lens`` and ``free_state`` (an
     update in place, e.g. inside a CUDA graph); by default they are new tensors.
     """
-    _require_cuda(page_table, lens, new_lens, free_pages, free_state, lens_out, free_state_out)
-    B, dev = lens.numel(), page_table.device
-    _same_device(dev, lens=lens, new_lens=new_lens, free_pages=free_pages, free_state=free_state, lens_out=lens_out,
-                 free_state_out=free_state_out)
-    _table("page_table", page_table, B)
+    if not page_table.is_cuda:
+        _bad_cuda()
+    index, dev = page_table.get_device(), page_table.device
+    B, ring = lens.numel(), free_pages.numel()
+    num_tokens = int(num_tokens)
+    if num_tokens < 0:
+        raise ValueError("num_tokens must not be negative")
+    a = L.SagaPageTableArgs()
+    a.B = B
+    a.page_len = int(page_len)
+    a.page_table = _table(page_table, index, B)
+    a.pt_sb = page_table.stride(0)
+    a.max_pages = page_table.shape[1]
+    a.lens = _ints("lens", lens, index, _I32, (B,))
+    a.new_lens = _ints("new_lens", new_lens, index, _I32, (B,))
+    a.free_pages = _ints("free_pages", free_pages, index, _I32, (ring,))
+    a.ring = ring
+    a.free_state = _ints("free_state", free_state, index, _I32, (2,))
     if lens_out is None:
         lens_out = torch.empty_like(lens)
     if free_state_out is None:
         free_state_out = torch.empty_like(free_state)
-    for name, t, shape in (("lens", lens, (B,)), ("new_lens", new_lens, (B,)), ("free_state", free_state, (2,)),
-                           ("free_pages", free_pages, (free_pages.numel(),)), ("lens_out", lens_out, (B,)),
-                           ("free_state_out", free_state_out, (2,))):
-        _int_tensor(name, t, torch.int32, shape)
-    num_tokens = int(num_tokens)
-    if num_tokens < 0:
-        raise ValueError("num_tokens must not be negative")
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    positions = torch.empty(num_tokens, dtype=torch.int32, device=dev)
-    offsets = torch.empty(B + 1, dtype=torch.int32, device=dev)
-    a = L.SagaPageTableArgs()
-    a.B, a.page_len, a.max_pages = B, int(page_len), page_table.shape[1]
-    a.page_table, a.pt_sb = page_table.data_ptr(), page_table.stride(0)
-    a.lens, a.new_lens = lens.data_ptr(), new_lens.data_ptr()
-    a.free_pages, a.ring, a.free_state = free_pages.data_ptr(), free_pages.numel(), free_state.data_ptr()
-    a.num_tokens, a.slots, a.positions = num_tokens, slots.data_ptr(), positions.data_ptr()
-    a.offsets, a.lens_out, a.free_state_out = offsets.data_ptr(), lens_out.data_ptr(), free_state_out.data_ptr()
-    a.status = status_tensor(dev).data_ptr()
-    with torch.cuda.device(dev):
-        ws = _scratch(dev, max(16 * B, 16))
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        L.check(L.lib.saga_page_tables(ctypes.byref(a), _stream(dev)), "saga_page_tables")
+    a.lens_out = _ints("lens_out", lens_out, index, _I32, (B,))
+    a.free_state_out = _ints("free_state_out", free_state_out, index, _I32, (2,))
+    slots = torch.empty(num_tokens, dtype=_I64, device=dev)
+    positions = torch.empty(num_tokens, dtype=_I32, device=dev)
+    offsets = torch.empty(B + 1, dtype=_I32, device=dev)
+    a.num_tokens = num_tokens
+    a.slots, a.positions, a.offsets = slots.data_ptr(), positions.data_ptr(), offsets.data_ptr()
+    a.status = _status(index)
+    nbytes = max(16 * B, 16)
+    with _on_device(index):
+        stream = _raw_stream(index)
+        a.workspace = _scratch(index, stream, nbytes)
+        a.workspace_bytes = nbytes
+        rc = L.lib.saga_page_tables(ctypes.byref(a), stream)
+    if rc:
+        L.check(rc, "saga_page_tables")
     return PageStep(slots, positions, offsets, lens_out, free_state_out)
 
 
@@ -306,21 +390,21 @@ def slot_map(page_table: torch.Tensor, lens: torch.Tensor, num_tokens: int, page
     """The slots (int64 [num_tokens]) of the positions [starts[b], lens[b]) that
     the requests already hold, packed in order of the requests, and their
     offsets (int32 [B + 1]). Rows beyond the last position get -1."""
-    _require_cuda(page_table, lens, starts)
-    B, dev = lens.numel(), page_table.device
-    _same_device(dev, lens=lens, starts=starts)
-    _table("page_table", page_table, B)
-    _int_tensor("lens", lens, torch.int32, (B,))
-    if starts is not None:
-        _int_tensor("starts", starts, torch.int32, (B,))
+    if not page_table.is_cuda:
+        _bad_cuda()
+    index, dev = page_table.get_device(), page_table.device
+    B = lens.numel()
+    table = _table(page_table, index, B)
+    at = _ints("lens", lens, index, _I32, (B,))
+    first = None if starts is None else _ints("starts", starts, index, _I32, (B,))
     num_tokens = int(num_tokens)
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    offsets = torch.empty(B + 1, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        L.check(L.lib.saga_slot_map(B, int(page_len), page_table.data_ptr(), page_table.stride(0),
-                                    page_table.shape[1], starts.data_ptr() if starts is not None else None,
-                                    lens.data_ptr(), num_tokens, slots.data_ptr(), offsets.data_ptr(),
-                                    status_tensor(dev).data_ptr(), _stream(dev)), "saga_slot_map")
+    slots = torch.empty(num_tokens, dtype=_I64, device=dev)
+    offsets = torch.empty(B + 1, dtype=_I32, device=dev)
+    with _on_device(index):
+        rc = L.lib.saga_slot_map(B, int(page_len), table, page_table.stride(0), page_table.shape[1], first, at,
+                                 num_tokens, slots.data_ptr(), offsets.data_ptr(), _status(index), _raw_stream(index))
+    if rc:
+        L.check(rc, "saga_slot_map")
     return slots, offsets
