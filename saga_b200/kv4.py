@@ -108,15 +108,43 @@ class Kv4Pool:
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("saga_b200 ops take CUDA tensors (there is no CPU path)")
-        self.num_pages, self.page_len = int(num_pages), int(page_len)
-        self.key_heads, self.value_heads, self.head_dim = int(key_heads), int(value_heads), int(head_dim)
-        self.k = torch.zeros((num_pages, key_heads, nbytes), dtype=torch.uint8, device=device)
-        self.v = torch.zeros((num_pages, value_heads, nbytes), dtype=torch.uint8, device=device)
-        self.device = self.k.device
-        self.k_lo = self.k_hi = None
+        k = torch.zeros((num_pages, key_heads, nbytes), dtype=torch.uint8, device=device)
+        v = torch.zeros((num_pages, value_heads, nbytes), dtype=torch.uint8, device=device)
+        lo = hi = None
         if bounds:
-            self.k_lo, self.k_hi = (torch.zeros((num_pages, key_heads, head_dim), dtype=torch.bfloat16,
-                                                device=self.device) for _ in range(2))
+            lo, hi = (torch.zeros((num_pages, key_heads, head_dim), dtype=torch.bfloat16, device=device)
+                      for _ in range(2))
+        self._bind(k, v, int(page_len), int(head_dim), lo, hi)
+
+    @classmethod
+    def of(cls, k: torch.Tensor, v: torch.Tensor, page_len: int, head_dim: int, k_lo: Optional[torch.Tensor] = None,
+           k_hi: Optional[torch.Tensor] = None) -> "Kv4Pool":
+        """The pool whose tensors these are (``pool.k``, ``pool.v``, ...)."""
+        nbytes = L.lib.saga_kv4_page_bytes(int(head_dim), int(page_len))
+        if nbytes == 0:
+            raise ValueError(L.lib.saga_last_error().decode())
+        if not (k.is_cuda and v.is_cuda):
+            _bad_cuda()
+        for name, t in (("k", k), ("v", v)):
+            if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != nbytes or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 [num_pages, heads, {nbytes}] tensor")
+        if k.device != v.device or k.shape[0] != v.shape[0]:
+            raise ValueError("k and v must share a device and num_pages")
+        if (k_lo is None) != (k_hi is None):
+            raise ValueError("k_lo and k_hi go together")
+        for name, t in (("k_lo", k_lo), ("k_hi", k_hi)):
+            if t is not None and not (t.dtype is torch.bfloat16 and t.device == k.device and t.is_contiguous()
+                                      and t.shape == (k.shape[0], k.shape[1], head_dim)):
+                raise ValueError(f"{name} must be a contiguous bfloat16 [num_pages, key_heads, head_dim] tensor")
+        pool = cls.__new__(cls)
+        pool._bind(k, v, int(page_len), int(head_dim), k_lo, k_hi)
+        return pool
+
+    def _bind(self, k, v, page_len, head_dim, k_lo, k_hi):
+        self.k, self.v, self.k_lo, self.k_hi = k, v, k_lo, k_hi
+        self.page_len, self.head_dim = page_len, head_dim
+        self.num_pages, self.key_heads, self.value_heads = k.shape[0], k.shape[1], v.shape[1]
+        self.device = k.device
         self._index = self.device.index
         self._desc = self.descriptor()
         self._ref = ctypes.byref(self._desc)
@@ -166,6 +194,8 @@ def kv4_write(pool: Kv4Pool, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
     (int64 [T]; -1 skips a row). A slot outside the pool sets
     ``STATUS_PAGE_RANGE`` and skips the row. In a pool with bounds, a page whose
     last slot is written gets its key bounds. Two rows must not name one slot."""
+    if torch.compiler.is_compiling():
+        return torch.ops.saga.kv4_write(*_tensors(pool), k, v, slots)
     T = _rows(pool, k, v, slots)
     ks, vs = k.stride(), v.stride()
     with _on_device(pool._index):
@@ -180,6 +210,8 @@ def kv4_read(pool: Kv4Pool, slots: torch.Tensor, dtype: torch.dtype = torch.bflo
     """What the slots stand for: ``k`` [T, Hk, D] and ``v`` [T, Hv, D] rounded
     to ``dtype``; zeros for slot -1 (and, with ``STATUS_PAGE_RANGE``, for a slot
     outside the pool). E.g. the history that a prompt chunk attends to."""
+    if torch.compiler.is_compiling():
+        return torch.ops.saga.kv4_read(*_tensors(pool), slots, dtype)
     T = slots.numel()
     code = _dtype_code(dtype)
     at = _ints("slots", slots, pool._index, _I64, (T,))
@@ -267,6 +299,8 @@ def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     zeros. With ``blocks`` and ``counts`` (``kv4_select``) each key head attends
     to those pages alone. ``scaling`` defaults to 1/sqrt(D).
     """
+    if torch.compiler.is_compiling():
+        return torch.ops.saga.kv4_decode(*_tensors(pool), query, page_table, lens, scaling, starts, blocks, counts)
     a = _kv4_args(query, pool, page_table, lens)
     B, Hq, D = a.B, a.Hq, pool.head_dim
     a.scaling = D ** -0.5 if scaling is None else float(scaling)
@@ -278,6 +312,8 @@ def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
         if blocks.dim() != 3:
             raise ValueError("blocks must be [B, Hk, top]")
         top = blocks.shape[2]
+        if top == 0:
+            raise ValueError("top must be positive (blocks is empty)")
         a.top = top
         a.blocks = _ints("blocks", blocks, pool._index, _I32, (B, pool.key_heads, top))
         a.counts = _ints("counts", counts, pool._index, _I32, (B, pool.key_heads))
@@ -301,6 +337,8 @@ def kv4_select(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     page is still filling) pages are always kept; ties go to the lower page;
     a request with at most ``top`` pages keeps them all.
     """
+    if torch.compiler.is_compiling():
+        return torch.ops.saga.kv4_select(*_tensors(pool), query, page_table, lens, top, keep_first, keep_last)
     a = _kv4_args(query, pool, page_table, lens)
     if pool.k_lo is None:
         raise ValueError("kv4_select needs a pool with bounds=True")
@@ -344,6 +382,14 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     ``lens_out`` and ``free_state_out`` may be ``lens`` and ``free_state`` (an
     update in place, e.g. inside a CUDA graph); by default they are new tensors.
     """
+    if torch.compiler.is_compiling():
+        step = PageStep(*torch.ops.saga.page_tables(page_table, lens, new_lens, free_pages, free_state, num_tokens,
+                                                    page_len))
+        if lens_out is not None:
+            step = step._replace(lens=lens_out.copy_(step.lens))
+        if free_state_out is not None:
+            step = step._replace(free_state=free_state_out.copy_(step.free_state))
+        return step
     if not page_table.is_cuda:
         _bad_cuda()
     index, dev = page_table.get_device(), page_table.device
@@ -408,3 +454,79 @@ def slot_map(page_table: torch.Tensor, lens: torch.Tensor, num_tokens: int, page
     if rc:
         L.check(rc, "saga_slot_map")
     return slots, offsets
+
+
+# ---------------------------------------------------------------------------
+# torch custom ops (opaque to torch.compile). A pool goes in as its tensors:
+# k, v, k_lo, k_hi, page_len, head_dim.
+# ---------------------------------------------------------------------------
+
+def _tensors(pool: Kv4Pool):
+    return pool.k, pool.v, pool.k_lo, pool.k_hi, pool.page_len, pool.head_dim
+
+
+@torch.library.custom_op("saga::kv4_write", mutates_args=("k_pool", "v_pool", "k_lo", "k_hi"))
+def _op_kv4_write(k_pool: torch.Tensor, v_pool: torch.Tensor, k_lo: Optional[torch.Tensor],
+                  k_hi: Optional[torch.Tensor], page_len: int, head_dim: int, k: torch.Tensor, v: torch.Tensor,
+                  slots: torch.Tensor) -> None:
+    kv4_write(Kv4Pool.of(k_pool, v_pool, page_len, head_dim, k_lo, k_hi), k, v, slots)
+
+
+@_op_kv4_write.register_fake
+def _(k_pool, v_pool, k_lo, k_hi, page_len, head_dim, k, v, slots):
+    return None
+
+
+@torch.library.custom_op("saga::kv4_read", mutates_args=())
+def _op_kv4_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_lo: Optional[torch.Tensor],
+                 k_hi: Optional[torch.Tensor], page_len: int, head_dim: int, slots: torch.Tensor,
+                 dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    return kv4_read(Kv4Pool.of(k_pool, v_pool, page_len, head_dim, k_lo, k_hi), slots, dtype)
+
+
+@_op_kv4_read.register_fake
+def _(k_pool, v_pool, k_lo, k_hi, page_len, head_dim, slots, dtype):
+    return tuple(t.new_empty((slots.numel(), t.shape[1], head_dim), dtype=dtype) for t in (k_pool, v_pool))
+
+
+@torch.library.custom_op("saga::kv4_decode", mutates_args=())
+def _op_kv4_decode(k_pool: torch.Tensor, v_pool: torch.Tensor, k_lo: Optional[torch.Tensor],
+                   k_hi: Optional[torch.Tensor], page_len: int, head_dim: int, query: torch.Tensor,
+                   page_table: torch.Tensor, lens: torch.Tensor, scaling: Optional[float],
+                   starts: Optional[torch.Tensor], blocks: Optional[torch.Tensor],
+                   counts: Optional[torch.Tensor]) -> torch.Tensor:
+    return kv4_decode(query, Kv4Pool.of(k_pool, v_pool, page_len, head_dim, k_lo, k_hi), page_table, lens, scaling,
+                      starts, blocks, counts)
+
+
+@_op_kv4_decode.register_fake
+def _(k_pool, v_pool, k_lo, k_hi, page_len, head_dim, query, page_table, lens, scaling, starts, blocks, counts):
+    return query.new_empty(query.shape)
+
+
+@torch.library.custom_op("saga::kv4_select", mutates_args=())
+def _op_kv4_select(k_pool: torch.Tensor, v_pool: torch.Tensor, k_lo: Optional[torch.Tensor],
+                   k_hi: Optional[torch.Tensor], page_len: int, head_dim: int, query: torch.Tensor,
+                   page_table: torch.Tensor, lens: torch.Tensor, top: int, keep_first: int,
+                   keep_last: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return kv4_select(query, Kv4Pool.of(k_pool, v_pool, page_len, head_dim, k_lo, k_hi), page_table, lens, top,
+                      keep_first, keep_last)
+
+
+@_op_kv4_select.register_fake
+def _(k_pool, v_pool, k_lo, k_hi, page_len, head_dim, query, page_table, lens, top, keep_first, keep_last):
+    rows = (query.shape[0], k_pool.shape[1])
+    return query.new_empty((*rows, top), dtype=torch.int32), query.new_empty(rows, dtype=torch.int32)
+
+
+@torch.library.custom_op("saga::page_tables", mutates_args=("page_table", "free_pages"))
+def _op_page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+                    free_state: torch.Tensor, num_tokens: int, page_len: int
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(page_tables(page_table, lens, new_lens, free_pages, free_state, num_tokens, page_len))
+
+
+@_op_page_tables.register_fake
+def _(page_table, lens, new_lens, free_pages, free_state, num_tokens, page_len):
+    return (lens.new_empty(num_tokens, dtype=torch.int64), lens.new_empty(num_tokens), lens.new_empty(lens.numel() + 1),
+            torch.empty_like(lens), torch.empty_like(free_state))
