@@ -270,7 +270,8 @@ typedef struct SagaKv4Pool {
   void* k; void* v;           /* page tiles, num_pages * H * page_len * (D/2 + D/16) bytes, 16-byte aligned */
   /* Optional key bounds (both or neither), bfloat16 [num_pages][Hk][D]: the
    * least and the greatest value that the page's keys stand for, per channel,
-   * rounded outwards. Taken when a page's last slot is written. */
+   * rounded outwards (NaN values left out; both NaN where all are). Taken when
+   * a page's last slot is written. */
   void* k_lo; void* k_hi;
 } SagaKv4Pool;
 
@@ -330,7 +331,8 @@ SAGA_API int saga_kv4_decode(const SagaKv4Args* args, void* stream);
  * the greatest, over the key head's queries, of sum_d q_d * (q_d > 0 ? hi_d :
  * lo_d), in binary32, summed by halves (d with d + D/2, then d + D/4, ...). The
  * first keep_first and the last keep_last pages of [0, lens[b]) are always
- * kept; of equal scores the lower page is kept; NaN counts as lowest. Requests
+ * kept; of equal scores the lower page is kept; a page with a NaN score is
+ * lowest. lo <= hi is assumed. Requests
  * with at most `top` pages keep them all. Needs the pool's bounds. */
 SAGA_API int saga_kv4_select(const SagaKv4Args* args, void* stream);
 

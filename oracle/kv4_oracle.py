@@ -50,11 +50,14 @@ def rows_value(x):
 
 
 def page_bounds(values):
-    """(lo, hi) per channel of a page's key values [page_len, D] (NaN rows left out), bfloat16 values."""
+    """(lo, hi) per channel of a page's key values [page_len, D] (NaN values left out; NaN where all are),
+    bfloat16 values."""
     v = np.asarray(values).astype(F32)
+    none = np.isnan(v).all(0)
     lo = np.where(np.isnan(v), F32(np.inf), v).min(0)
     hi = np.where(np.isnan(v), F32(-np.inf), v).max(0)
-    return bf16_towards(lo, False), bf16_towards(hi, True)
+    return tuple(np.where(none, F32("nan"), b) for b in (bf16_towards(np.where(none, 0, lo), False),
+                                                         bf16_towards(np.where(none, 0, hi), True)))
 
 
 def block_score(q, lo, hi):

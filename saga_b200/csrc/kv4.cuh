@@ -44,6 +44,31 @@ __device__ __forceinline__ int64_t kv4_tile_at(int64_t page, int h, int H, int o
   return ((page * H + h) * (int64_t)(page_len / kKv4Tile) + off / kKv4Tile) * kv4_tile_bytes(D);
 }
 
+// Two binary32 values in one register pair: the packed forms issue one instruction for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // The greatest bfloat16 at or below x, the least at or above it.
 __device__ __forceinline__ __nv_bfloat16 bf16_down(float x) { return __float2bfloat16_rd(x); }
 __device__ __forceinline__ __nv_bfloat16 bf16_up(float x) { return __float2bfloat16_ru(x); }

@@ -1,37 +1,91 @@
 // Quantised writes into the 4-bit paged cache, reads of what it stands for, and
 // the key bounds of completed pages.
+#include <algorithm>
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace saga {
 
 namespace {
 
-// Eight lanes hold one group: lane l has its values 8l .. 8l + 7, so a row's
-// 16-bit values arrive in 16-byte loads and leave as one word of codes per lane,
-// 32 consecutive bytes (one sector) per group.
-constexpr int kLanesPerGroup = 8;
+// Four lanes hold one group: lane l has its values 8l .. 8l + 7 and 32 + 8l ..
+// 39 + 8l, so that 16-bit values arrive in 16-byte loads of 64 consecutive bytes
+// per group and leave as two words of codes per lane, 32 consecutive bytes (one
+// sector) per group. What is done once per group (the address, the scale) costs
+// as much as ten values, so fewer lanes with more values each are cheaper: eight
+// lanes of eight values took 98 us where these take 56 us (131,072 tokens, five
+// heads of 128, bf16: 215 MB).
+constexpr int kLanes = 4;
+constexpr int kCtaThreads = 256;
+constexpr int kCtaGroups = kCtaThreads / kLanes;
+constexpr int kAhead = 2;  // groups that a lane loads before it works on the first
 
+// Sixteen values of a lane as they are loaded.
+template <typename T>
+struct Raw {
+  uint4 w[sizeof(T)];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float* f) {
-  if constexpr (VEC) {
-    load8f<T>(p, f);
-  } else {
+__device__ __forceinline__ void load16(const T* p, Raw<T>& r) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Num<T>::to_f(p[i]);
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        r.w[h * sizeof(T) / 2 + i] = reinterpret_cast<const uint4*>(p + 32 * h)[i];
+    } else {
+      T* t = reinterpret_cast<T*>(&r) + 8 * h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = p[32 * h + i];
+    }
   }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, const float* f) {
-  T t[8];
+__device__ __forceinline__ void store16(T* p, const Raw<T>& r) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = Num<T>::from_f(f[i]);
-  if constexpr (VEC) {
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4*>(p + 32 * h)[i] = r.w[h * sizeof(T) / 2 + i];
+    } else {
+      const T* t = reinterpret_cast<const T*>(&r) + 8 * h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[32 * h + i] = t[i];
+    }
+  }
+}
+
+// Least and greatest of a lane's sixteen values, and a value that is not 0 if
+// one of them is NaN or infinite. The 16-bit types are compared in pairs.
+template <typename T>
+__device__ __forceinline__ void extremes(const Raw<T>& r, float& lo, float& hi, float& odd) {
+  if constexpr (sizeof(T) == 4) {
+    const float* x = reinterpret_cast<const float*>(&r);
+    lo = hi = x[0];
+    odd = x[0] * 0.f;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+      odd = fmaf(x[i], 0.f, odd);
+    }
   } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* x = reinterpret_cast<const T2*>(&r);
+    T2 zero;
+    *reinterpret_cast<uint32_t*>(&zero) = 0u;
+    T2 a = x[0], b = x[0], o = __hmul2(x[0], zero);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = t[i];
+    for (int i = 1; i < 8; ++i) {
+      a = __hmin2(a, x[i]);
+      b = __hmax2(b, x[i]);
+      o = __hfma2(x[i], zero, o);
+    }
+    lo = fminf(Num<T>::to_f(a.x), Num<T>::to_f(a.y));
+    hi = fmaxf(Num<T>::to_f(b.x), Num<T>::to_f(b.y));
+    odd = Num<T>::to_f(o.x) + Num<T>::to_f(o.y);
   }
 }
 
@@ -41,109 +95,158 @@ struct Rows {  // keys or values, [T, H, D]
   int H;
 };
 
-// The group of eight lanes that the calling thread belongs to handles unit u:
-// token u / (H * NG), head and group from the rest.
-template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(256) kv4_write_kernel(const T* __restrict__ k, const T* __restrict__ v, Rows kr,
-                                                        Rows vr, int64_t T_, const int64_t* __restrict__ slots,
-                                                        int page_len, int num_pages, int* status) {
-  pdl_wait();
+// How the groups of T tokens are dealt out: a CTA has `strip` tokens, all heads
+// and groups of each; `magic` divides by the groups of a token.
+struct Deal {
+  int64_t T;
+  int strip, per;
+  uint32_t magic;
+  int tpp_shift;   // log2 of the tiles per page
+  int64_t slots;   // of the pool
+};
+
+// Unit u of the CTA's strip: its values, and the tile of its slot if that is in
+// the pool.
+template <int D>
+struct Unit {
+  uint8_t* tile;  // NULL: no slot
+  int64_t src;    // element offset of the lane's values in the tensor
+  int row, g;
+  bool is_v;
+  bool live;  // the token exists
+};
+template <int D>
+__device__ __forceinline__ Unit<D> locate_unit(uint32_t u, const Deal& d, const Rows& kr, const Rows& vr,
+                                               const int64_t* __restrict__ slots, int l, int* status) {
   constexpr int NG = D / 64;
-  const int l = threadIdx.x & (kLanesPerGroup - 1);
-  const int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanesPerGroup;
-  const int per = (kr.H + vr.H) * NG;
-  const int64_t t = u / per;
-  // lanes past the end keep taking part in the shuffles below
-  int64_t slot = t < T_ ? slots[t] : -1;
-  const int rest = (int)(u - t * per);
-  const int g = rest % NG;
+  Unit<D> x;
+  const uint32_t tl = __umulhi(u, d.magic);  // u / per
+  const int rest = (int)(u - tl * (uint32_t)d.per);
+  const int64_t t = (int64_t)blockIdx.x * d.strip + tl;
+  x.live = (int)tl < d.strip && t < d.T;
+  const int64_t slot = x.live ? slots[t] : -1;
+  x.g = rest % NG;
   int h = rest / NG;
-  if (slot < 0 || slot >= (int64_t)num_pages * page_len) {
-    if (slot != -1 && rest == 0 && l == 0) set_status(status, SAGA_STATUS_PAGE_RANGE);
-    slot = -1;
-  }
-  const bool is_v = h >= kr.H;
-  if (is_v) h -= kr.H;
-  const Rows r = is_v ? vr : kr;
-  float x[8];
+  x.is_v = h >= kr.H;
+  if (x.is_v) h -= kr.H;
+  x.src = t * (x.is_v ? vr.st : kr.st) + h * (x.is_v ? vr.sh : kr.sh) + x.g * 64 + l * 8;
+  const bool inside = slot >= 0 && slot < d.slots;
+  if (!inside && slot != -1 && rest == 0 && l == 0) set_status(status, SAGA_STATUS_PAGE_RANGE);
+  x.row = (int)slot & (kKv4Tile - 1);
+  const uint32_t ptile = (uint32_t)(slot / kKv4Tile);  // the host checks that the pool's tiles fit an int
+  const uint32_t page = ptile >> d.tpp_shift, in_page = ptile & ((1u << d.tpp_shift) - 1u);
+  const int64_t tile = (((int64_t)page * (x.is_v ? vr.H : kr.H) + h) << d.tpp_shift) + in_page;
+  x.tile = inside ? (x.is_v ? vr.pool : kr.pool) + tile * kv4_tile_bytes(D) : nullptr;
+  return x;
+}
+// Where a lane's words of codes are: 8l .. 8l + 7 of the group in its first, 32 further in its second chunk.
+template <int D>
+__device__ __forceinline__ uint32_t* code_word(const Unit<D>& x, int h, int l) {
+  return reinterpret_cast<uint32_t*>(x.tile + kv4_chunk_off<D>(x.row, x.g * 2 + h) + l * 4);
+}
+
+constexpr float kMagic = 8388608.f;  // 2^23: adding it rounds to a whole number, to nearest even
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(kCtaThreads) kv4_write_kernel(const T* __restrict__ k, const T* __restrict__ v,
+                                                                Rows kr, Rows vr, Deal deal,
+                                                                const int64_t* __restrict__ slots, int* status) {
+  pdl_wait();
+  const int l = threadIdx.x & (kLanes - 1);
+  const uint32_t units = (uint32_t)deal.strip * (uint32_t)deal.per;
+  const unsigned lanes = 0xfu << (threadIdx.x & 28);
+  for (uint32_t u0 = 0; u0 < units; u0 += kCtaGroups * kAhead) {  // the same trips for all lanes of a warp
+    Unit<D> at[kAhead];
+    Raw<T> raw[kAhead];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (slot >= 0) load8<T, VEC>((is_v ? v : k) + t * r.st + h * r.sh + g * 64 + l * 8, x);
-  float lo = x[0], hi = x[0];
-  bool bad = !isfinite(x[0]);
+    for (int i = 0; i < kAhead; ++i) {
+      at[i] = locate_unit<D>(u0 + i * kCtaGroups + threadIdx.x / kLanes, deal, kr, vr, slots, l, status);
+      raw[i] = Raw<T>();
+      if (at[i].tile) load16<T, VEC>((at[i].is_v ? v : k) + at[i].src, raw[i]);
+    }
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad |= !isfinite(x[i]);
-  }
+    for (int i = 0; i < kAhead; ++i) {
+      float lo, hi, odd;
+      extremes<T>(raw[i], lo, hi, odd);
 #pragma unroll
-  for (int o = kLanesPerGroup / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  const unsigned lanes = 0xffu << (threadIdx.x & 24);
-  bad = (__ballot_sync(0xffffffffu, bad) & lanes) != 0;
-  // rounded down and up, so that z and z + 15 s enclose the group
-  const __nv_bfloat16 zb = bf16_down(lo);
-  const float z = __bfloat162float(zb);
-  const __nv_bfloat16 sb = bf16_up(fmaxf(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f), 0x1p-40f));
-  const float s = __bfloat162float(sb);
-  bad = bad || !isfinite(z) || !isfinite(s);
-  const float inv = __frcp_rn(s);
-  uint32_t w = 0;
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      // rounded down and up, so that z and z + 15 s enclose the group
+      const __nv_bfloat16 zb = bf16_down(lo);
+      const float z = __bfloat162float(zb);
+      const __nv_bfloat16 sb = bf16_up(fmaxf(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f), 0x1p-40f));
+      const float s = __bfloat162float(sb);
+      const bool bad = (__ballot_sync(0xffffffffu, odd != 0.f) & lanes) != 0 || !isfinite(z) || !isfinite(s);
+      const float inv = __frcp_rn(s);
+      // (x - z) / s lies in [0, 15] but for its rounding, so the nearest whole number is a code without
+      // a clamp. It is rounded by adding 2^23; the words 0x4b000000 + code are summed at their places
+      // and what the constants amount to is taken off.
+      const f32x2 minus_z = pack2(-z, -z);
+      constexpr uint32_t kOff = 0x4b000000u + (0x4b000000u << 4);  // the higher places overflow
+      const T* x = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], z), inv)), 0.f), 15.f);
-    w |= (uint32_t)c << (4 * i);
-  }
-  if (slot < 0) return;
-  const int off = (int)(slot & (page_len - 1));
-  uint8_t* tile = r.pool + kv4_tile_at<D>(slot / page_len, h, r.H, off, page_len);
-  const int row = off % kKv4Tile;
-  *reinterpret_cast<uint32_t*>(tile + kv4_chunk_off<D>(row, g * 2 + (l >> 2)) + (l & 3) * 4) = bad ? 0u : w;
-  if (l == 0) {
-    const uint32_t m = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
-    *reinterpret_cast<uint32_t*>(tile + kv4_meta_off<D>(row, g)) = bad ? 0x7fff7fffu : m;
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          float y0, y1;
+          unpack2(add2(pack2(Num<T>::to_f(x[8 * h + j]), Num<T>::to_f(x[8 * h + j + 1])), minus_z), y0, y1);
+          // not packed: the assembler joins a packed product with the packed sum after it
+          w += __float_as_uint(__fadd_rn(__fmul_rn(y0, inv), kMagic)) << (4 * j);
+          w += __float_as_uint(__fadd_rn(__fmul_rn(y1, inv), kMagic)) << (4 * j + 4);
+        }
+        if (at[i].tile) *code_word<D>(at[i], h, l) = bad ? 0u : w - kOff;
+      }
+      if (l == 0 && at[i].tile) {
+        const uint32_t m = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+        *reinterpret_cast<uint32_t*>(at[i].tile + kv4_meta_off<D>(at[i].row, at[i].g)) = bad ? 0x7fff7fffu : m;
+      }
+    }
   }
 }
 
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(256) kv4_read_kernel(T* __restrict__ k, T* __restrict__ v, Rows kr, Rows vr,
-                                                       int64_t T_, const int64_t* __restrict__ slots, int page_len,
-                                                       int num_pages, int* status) {
+__global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k, T* __restrict__ v, Rows kr, Rows vr,
+                                                               Deal deal, const int64_t* __restrict__ slots,
+                                                               int* status) {
   pdl_wait();
-  constexpr int NG = D / 64;
-  const int l = threadIdx.x & (kLanesPerGroup - 1);
-  const int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanesPerGroup;
-  const int per = (kr.H + vr.H) * NG;
-  const int64_t t = u / per;
-  if (t >= T_) return;
-  const int64_t slot = slots[t];
-  const int rest = (int)(u - t * per);
-  const int g = rest % NG;
-  int h = rest / NG;
-  const bool is_v = h >= kr.H;
-  if (is_v) h -= kr.H;
-  const Rows r = is_v ? vr : kr;
-  float x[8];
-  if (slot < 0 || slot >= (int64_t)num_pages * page_len) {
-    if (slot != -1 && rest == 0 && l == 0) set_status(status, SAGA_STATUS_PAGE_RANGE);
+  const int l = threadIdx.x & (kLanes - 1);
+  const uint32_t units = (uint32_t)deal.strip * (uint32_t)deal.per;
+  for (uint32_t u0 = 0; u0 < units; u0 += kCtaGroups * kAhead) {
+    Unit<D> at[kAhead];
+    uint32_t w[kAhead][2], m[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  } else {
-    const int off = (int)(slot & (page_len - 1));
-    const uint8_t* tile = r.pool + kv4_tile_at<D>(slot / page_len, h, r.H, off, page_len);
-    const int row = off % kKv4Tile;
-    const uint32_t w =
-        *reinterpret_cast<const uint32_t*>(tile + kv4_chunk_off<D>(row, g * 2 + (l >> 2)) + (l & 3) * 4);
-    const uint32_t m = *reinterpret_cast<const uint32_t*>(tile + kv4_meta_off<D>(row, g));
-    const float s = kv4_scale(m), z = kv4_zero(m);
-    // s * code has at most 12 significant bits, so the sum is rounded once
+    for (int i = 0; i < kAhead; ++i) {
+      at[i] = locate_unit<D>(u0 + i * kCtaGroups + threadIdx.x / kLanes, deal, kr, vr, slots, l, status);
+      w[i][0] = w[i][1] = m[i] = 0u;
+      if (at[i].tile) {
+        w[i][0] = *code_word<D>(at[i], 0, l);
+        w[i][1] = *code_word<D>(at[i], 1, l);
+        m[i] = *reinterpret_cast<const uint32_t*>(at[i].tile + kv4_meta_off<D>(at[i].row, at[i].g));
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmaf_rn(s, (float)((w >> (4 * i)) & 15u), z);
+    for (int i = 0; i < kAhead; ++i) {
+      if (!at[i].live) continue;
+      const float s = kv4_scale(m[i]), z = kv4_zero(m[i]);
+      Raw<T> r;
+      T* x = reinterpret_cast<T*>(&r);
+      const f32x2 s2 = pack2(s, s), z2 = pack2(z, z), magic = pack2(-kMagic, -kMagic);
+      // s * code has at most 12 significant bits, so the sum is rounded once
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const uint32_t c = w[i][j / 8] >> (4 * (j % 8));
+        const f32x2 y = pack2(__uint_as_float((c & 15u) | 0x4b000000u), __uint_as_float(((c >> 4) & 15u) | 0x4b000000u));
+        float y0, y1;
+        unpack2(fma2(s2, add2(y, magic), z2), y0, y1);
+        x[j] = Num<T>::from_f(y0);
+        x[j + 1] = Num<T>::from_f(y1);
+      }
+      store16<T, VEC>((at[i].is_v ? v : k) + at[i].src, r);
+    }
   }
-  store8<T, VEC>((is_v ? v : k) + t * r.st + h * r.sh + g * 64 + l * 8, x);
 }
 
 // Bounds of the pages whose last slot is among the slots: a CTA looks at
@@ -155,12 +258,22 @@ __global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t 
   constexpr int W = D / 8, ROWS = 128 / W;
   __shared__ float red[2][ROWS][D];
   pdl_wait();
+  __shared__ int64_t done[32];
+  __shared__ int n_done;
   const int w = threadIdx.x % W, rr = threadIdx.x / W;
-  for (int64_t t = (int64_t)blockIdx.x * strip; t < min((int64_t)(blockIdx.x + 1) * strip, T_); ++t) {
-    const int64_t slot = slots[t];
-    if (slot < 0 || slot >= (int64_t)p.num_pages * p.page_len || (slot & (p.page_len - 1)) != p.page_len - 1)
-      continue;
-    const int64_t page = slot / p.page_len;
+  if (threadIdx.x < 32) {  // strip <= 32
+    const int64_t t = (int64_t)blockIdx.x * strip + threadIdx.x;
+    const int64_t slot = (int)threadIdx.x < strip && t < T_ ? slots[t] : -1;
+    const bool last = slot >= 0 && slot < (int64_t)p.num_pages * p.page_len &&
+                      (slot & (p.page_len - 1)) == p.page_len - 1;
+    const unsigned all = __ballot_sync(0xffffffffu, last);
+    if (last) done[__popc(all & ((1u << threadIdx.x) - 1u))] = slot / p.page_len;
+    if (threadIdx.x == 0) n_done = __popc(all);
+  }
+  __syncthreads();
+  const int n = n_done;
+  for (int x = 0; x < n; ++x) {
+    const int64_t page = done[x];
     for (int h = 0; h < p.Hk; ++h) {
       float lo[8], hi[8];
 #pragma unroll
@@ -168,6 +281,7 @@ __global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t 
         lo[i] = INFINITY;
         hi[i] = -INFINITY;
       }
+#pragma unroll 4
       for (int off = rr; off < p.page_len; off += ROWS) {
         const uint8_t* tile =
             reinterpret_cast<const uint8_t*>(p.k) + kv4_tile_at<D>(page, h, p.Hk, off, p.page_len);
@@ -178,7 +292,7 @@ __global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t 
         const float s = kv4_scale(m), z = kv4_zero(m);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // NaN rows are left out (fminf and fmaxf return the other operand)
-          const float x = __fmaf_rn(s, (float)((c >> (4 * i)) & 15u), z);
+          const float x = __fmaf_rn(s, __uint_as_float(((c >> (4 * i)) & 15u) | 0x4b000000u) - kMagic, z);
           lo[i] = fminf(lo[i], x);
           hi[i] = fmaxf(hi[i], x);
         }
@@ -196,6 +310,7 @@ __global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t 
           a = fminf(a, red[0][i][threadIdx.x]);
           b = fmaxf(b, red[1][i][threadIdx.x]);
         }
+        if (a > b) a = b = __int_as_float(0x7fffffff);  // no key stands for a number here
         const int64_t at = (page * p.Hk + h) * D + threadIdx.x;
         reinterpret_cast<__nv_bfloat16*>(p.k_lo)[at] = bf16_down(a);
         reinterpret_cast<__nv_bfloat16*>(p.k_hi)[at] = bf16_up(b);
@@ -228,23 +343,43 @@ void dispatch(int dt, int D, bool vec, F f) {
 
 }  // namespace
 
+// A CTA's strip is cut so that its groups fill all lanes kAhead deep about
+// twice, or to one token where there are too few tokens to fill the SMs so.
+static int make_deal(const SagaKv4Pool& p, int64_t T, Deal* d, unsigned* grid) {
+  d->T = T;
+  d->per = (p.Hk + p.Hv) * (p.D / 64);
+  const int full = std::max(1, 2 * kAhead * kCtaGroups / d->per);
+  d->strip = (int)std::max<int64_t>(1, std::min<int64_t>(full, T / (2 * 148)));
+  // exact for u * per < 2^32; u stays below strip * per + 2 kAhead kCtaGroups
+  d->magic = (uint32_t)(((1ull << 32) + d->per - 1) / d->per);
+  if ((uint64_t)((int64_t)d->strip * d->per + 2 * kAhead * kCtaGroups) * d->per >= (1ull << 32) || d->per < 2)
+    return abi_fail(SAGA_ERR_UNSUPPORTED, "too many heads");
+  d->tpp_shift = 0;
+  while ((kKv4Tile << d->tpp_shift) < p.page_len) ++d->tpp_shift;
+  d->slots = (int64_t)p.num_pages * p.page_len;
+  const int64_t n = (T + d->strip - 1) / d->strip;
+  if (n > 0x7fffffffll) return abi_fail(SAGA_ERR_UNSUPPORTED, "too many rows for one call");
+  *grid = (unsigned)n;
+  return SAGA_OK;
+}
+
 int launch_kv4_write(const SagaKv4Pool& p, int dt, int64_t T, const void* k, int64_t k_st, int64_t k_sh,
                      const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots, int* status, cudaStream_t st) {
   const int esz = dt == SAGA_FP32 ? 4 : 2;
   const bool vec = rows_aligned(k, k_st, k_sh, esz) && rows_aligned(v, v_st, v_sh, esz);
   const Rows kr{k_st, k_sh, reinterpret_cast<uint8_t*>(p.k), p.Hk};
   const Rows vr{v_st, v_sh, reinterpret_cast<uint8_t*>(p.v), p.Hv};
-  const int64_t threads = T * (p.Hk + p.Hv) * (p.D / 64) * kLanesPerGroup;
-  const int64_t grid = (threads + 255) / 256;
-  if (grid > 0x7fffffffll) return abi_fail(SAGA_ERR_UNSUPPORTED, "too many rows for one call");
-  int rc = SAGA_OK;
+  Deal deal;
+  unsigned grid;
+  int rc = make_deal(p, T, &deal, &grid);
+  if (rc) return rc;
   dispatch(dt, p.D, vec, [&](auto* t, auto d, auto a) {
     using E = std::remove_pointer_t<decltype(t)>;
-    rc = kv4_launch("kv4_write_kernel", kv4_write_kernel<E, d.value, a.value>, dim3((unsigned)grid), 256, 0, st,
-                    reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v), kr, vr, T, slots, p.page_len,
-                    p.num_pages, status);
+    rc = kv4_launch("kv4_write_kernel", kv4_write_kernel<E, d.value, a.value>, dim3(grid), kCtaThreads, 0, st,
+                    reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v), kr, vr, deal, slots, status);
   });
   if (rc || !p.k_lo) return rc;
+  // one token per CTA where every token may complete a page; runs of prompt tokens complete one in 32 at most
   const int strip = T <= 4096 ? 1 : 32;
   const unsigned nb = (unsigned)((T + strip - 1) / strip);
   return kv4_launch("kv4_bounds_kernel", p.D == 128 ? kv4_bounds_kernel<128> : kv4_bounds_kernel<64>, dim3(nb), 128, 0,
@@ -257,15 +392,14 @@ int launch_kv4_read(const SagaKv4Pool& p, int dt, int64_t T, const int64_t* slot
   const bool vec = rows_aligned(k, k_st, k_sh, esz) && rows_aligned(v, v_st, v_sh, esz);
   const Rows kr{k_st, k_sh, reinterpret_cast<uint8_t*>(p.k), p.Hk};
   const Rows vr{v_st, v_sh, reinterpret_cast<uint8_t*>(p.v), p.Hv};
-  const int64_t threads = T * (p.Hk + p.Hv) * (p.D / 64) * kLanesPerGroup;
-  const int64_t grid = (threads + 255) / 256;
-  if (grid > 0x7fffffffll) return abi_fail(SAGA_ERR_UNSUPPORTED, "too many rows for one call");
-  int rc = SAGA_OK;
+  Deal deal;
+  unsigned grid;
+  int rc = make_deal(p, T, &deal, &grid);
+  if (rc) return rc;
   dispatch(dt, p.D, vec, [&](auto* t, auto d, auto a) {
     using E = std::remove_pointer_t<decltype(t)>;
-    rc = kv4_launch("kv4_read_kernel", kv4_read_kernel<E, d.value, a.value>, dim3((unsigned)grid), 256, 0, st,
-                    reinterpret_cast<E*>(k), reinterpret_cast<E*>(v), kr, vr, T, slots, p.page_len, p.num_pages,
-                    status);
+    rc = kv4_launch("kv4_read_kernel", kv4_read_kernel<E, d.value, a.value>, dim3(grid), kCtaThreads, 0, st,
+                    reinterpret_cast<E*>(k), reinterpret_cast<E*>(v), kr, vr, deal, slots, status);
   });
   return rc;
 }

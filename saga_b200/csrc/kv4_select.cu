@@ -14,42 +14,41 @@ namespace saga {
 namespace {
 
 constexpr int kTopThreads = 512;
-constexpr int kTopKeys = 8192;  // keys kept in shared memory; further ones are made again from the scores
+constexpr int kTopKeys = 8192;  // keys kept in shared memory; further ones are read again
 
-// Order-preserving key of a score: NaN lowest, -0 as +0; 0 is below every score.
+// Order-preserving key of a score, -0 as +0; kNanKey is below every number's and 0 below that.
+constexpr uint32_t kNanKey = 1u;
 __device__ __forceinline__ uint32_t score_key(float x) {
-  if (x != x) return 1u;
   const uint32_t u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Sums v[0..NV-1] over the warp, value by value in the same tree as a butterfly
-// from distance 16 down to 1, halving the live values at each step: lane l ends
-// with the sum of value l / (32 / NV).
-template <int NV>
-__device__ __forceinline__ float warp_sums(float (&v)[NV]) {
+// Sums v[0..3] over the warp, each in the same tree as a butterfly from distance
+// 16 down to 1, halving the live values at the first two steps: lane l ends with
+// the sum of value l / 8.
+__device__ __forceinline__ float warp_sums4(float (&v)[4]) {
   const int lane = threadIdx.x & 31;
-  int o = 16;
+  bool up = (lane & 16) != 0;
 #pragma unroll
-  for (int n = NV / 2; n > 0; n >>= 1, o >>= 1) {
-    const bool up = (lane & o) != 0;
+  for (int i = 0; i < 2; ++i)
+    v[i] = __fadd_rn(up ? v[i + 2] : v[i], __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + 2], 16));
+  up = (lane & 8) != 0;
+  float s = __fadd_rn(up ? v[1] : v[0], __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 8));
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float send = up ? v[i] : v[i + n];
-      v[i] = __fadd_rn(up ? v[i + n] : v[i], __shfl_xor_sync(0xffffffffu, send, o));
-    }
-  }
-#pragma unroll
-  for (; o > 0; o >>= 1) v[0] = __fadd_rn(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
-  return v[0];
+  for (int o = 4; o > 0; o >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, o));
+  return s;
 }
 
-// A warp scores one page at a time for the heads of one key head, NV at a time
-// in registers: lane l has channels l, l + 32 (l + 64, l + 96), so the first
-// levels of the tree are its own and the last five go across the warp.
-template <typename T, int D, int NV>
-__global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, float* __restrict__ scores) {
-  constexpr int N = D / 32;
+constexpr int kScorePages = 4;  // pages per warp, at most
+
+// A warp scores `per_warp` consecutive pages for the heads of one key head, 4 NC
+// of them at a time in registers: lane l has channels l, l + 32 (l + 64, l + 96),
+// so the first levels of the tree are its own and the last five go across the
+// warp. Scores are written as keys.
+template <typename T, int D, int NC>
+__global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, uint32_t* __restrict__ keys, int per_warp) {
+  constexpr int N = D / 32, NV = 4 * NC;
+  __shared__ float qs[NV][D];
   pdl_wait();
   const int G = a.Hq / a.pool.Hk;
   const int row = blockIdx.y;
@@ -58,77 +57,100 @@ __global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, float* __
   const int pl = a.pool.page_len;
   const int len = min(max(a.lens[b], 0), a.max_pages * pl);
   const int pages = (len + pl - 1) / pl;
-  if (pages <= a.top) return;  // all are kept
-  const int step = gridDim.x * (blockDim.x >> 5);
   // the kept pages at either end need no score
-  const int j0 = a.keep_first + blockIdx.x * (blockDim.x >> 5) + warp, j1 = pages - a.keep_last;
-  if (j0 >= j1) return;
+  const int c0 = a.keep_first + (int)blockIdx.x * 8 * per_warp, j1 = pages - a.keep_last;
+  if (pages <= a.top || c0 >= j1) return;  // all are kept, or the row ends before this CTA
+  const int j0 = c0 + warp * per_warp;
+  const int n = min(per_warp, j1 - j0);
+  int mine = 0;  // lane i has the warp's i-th page
+  if (lane < n) {
+    mine = a.page_table[(int64_t)b * a.pt_sb + j0 + lane];
+    if (mine < 0 || mine >= a.pool.num_pages) {
+      set_status(a.status, SAGA_STATUS_PAGE_RANGE);
+      mine = 0;
+    }
+  }
+  // the bounds of all its pages are on their way while the queries are staged
+  __nv_bfloat16 lo[kScorePages][N], hi[kScorePages][N];
+#pragma unroll
+  for (int x = 0; x < kScorePages; ++x) {
+    const int page = __shfl_sync(0xffffffffu, mine, x);
+    if (x < n) {
+      const int64_t at = ((int64_t)page * a.pool.Hk + kh) * D + lane;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        lo[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_lo)[at + 32 * i];
+        hi[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_hi)[at + 32 * i];
+      }
+    }
+  }
   const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)kh * G * a.q_sh;
+  uint32_t best[kScorePages];
+#pragma unroll
+  for (int x = 0; x < kScorePages; ++x) best[x] = 0u;
+  bool nan[kScorePages] = {};
   for (int g0 = 0; g0 < G; g0 += NV) {
-    float qv[NV][N];
+    // one coalesced load of the queries per CTA: a warp's own 2-byte loads of all heads took longer than its pages
+    __syncthreads();
+    for (int x = threadIdx.x; x < NV * D; x += 256) {
+      const int g = x / D, d = x % D;
+      qs[g][d] = g0 + g < G ? Num<T>::to_f(q[(int64_t)(g0 + g) * a.q_sh + d]) : 0.f;
+    }
+    __syncthreads();
+    f32x2 qv[NV][N / 2];
 #pragma unroll
     for (int g = 0; g < NV; ++g)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        qv[g][i] = g0 + g < G ? Num<T>::to_f(q[(int64_t)(g0 + g) * a.q_sh + lane + 32 * i]) : 0.f;
-    // pages of this warp: lane i finds the i-th of the next 32
-    for (int base = j0; base < j1; base += 32 * step) {
-      int mine = 0;
-      if (base + lane * step < j1) {
-        mine = a.page_table[(int64_t)b * a.pt_sb + base + lane * step];
-        if (mine < 0 || mine >= a.pool.num_pages) {
-          set_status(a.status, SAGA_STATUS_PAGE_RANGE);
-          mine = 0;
-        }
+      for (int i = 0; i < N / 2; ++i) qv[g][i] = pack2(qs[g][lane + 64 * i], qs[g][lane + 64 * i + 32]);
+#pragma unroll
+    for (int x = 0; x < kScorePages; ++x) {
+      if (x >= n) break;
+      f32x2 l[N / 2], h[N / 2];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        l[i] = pack2(__bfloat162float(lo[x][2 * i]), __bfloat162float(lo[x][2 * i + 1]));
+        h[i] = pack2(__bfloat162float(hi[x][2 * i]), __bfloat162float(hi[x][2 * i + 1]));
       }
-      const int n = min(32, (j1 - base + step - 1) / step);
-      __nv_bfloat16 lo[N], hi[N];
-      auto fetch = [&](int x) {
-        const int page = __shfl_sync(0xffffffffu, mine, x);
-        const int64_t at = ((int64_t)page * a.pool.Hk + kh) * D + lane;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          lo[i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_lo)[at + 32 * i];
-          hi[i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_hi)[at + 32 * i];
+      for (int c = 0; c < NC; ++c) {
+        float s[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          // lo <= hi, so the greater of the two products is the one that the sign of q picks
+          f32x2 y[N / 2];
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) {
+            float h0, h1, l0, l1;
+            unpack2(mul2(qv[4 * c + g][i], h[i]), h0, h1);
+            unpack2(mul2(qv[4 * c + g][i], l[i]), l0, l1);
+            y[i] = pack2(fmaxf(h0, l0), fmaxf(h1, l1));
+          }
+          if constexpr (N == 4) y[0] = add2(y[0], y[N / 2 - 1]);  // channels d and d + 64
+          float y0, y1;
+          unpack2(y[0], y0, y1);
+          s[g] = __fadd_rn(y0, y1);  // d and d + 32
         }
-      };
-      fetch(0);
-      for (int x = 0; x < n; ++x) {
-        float l[N], h[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          l[i] = __bfloat162float(lo[i]);
-          h[i] = __bfloat162float(hi[i]);
-        }
-        if (x + 1 < n) fetch(x + 1);
-        float s[NV];
-#pragma unroll
-        for (int g = 0; g < NV; ++g) {
-          float y[N];
-#pragma unroll
-          for (int i = 0; i < N; ++i) y[i] = __fmul_rn(qv[g][i], qv[g][i] > 0.f ? h[i] : l[i]);
-#pragma unroll
-          for (int m = N / 2; m > 0; m >>= 1)
-#pragma unroll
-            for (int i = 0; i < m; ++i) y[i] = __fadd_rn(y[i], y[i + m]);
-          s[g] = y[0];
-        }
-        float best = warp_sums<NV>(s);
-        if (g0 + lane / (32 / NV) >= G) best = -INFINITY;
-        best = warp_nanmax(best);
-        if (lane == 0) {
-          float* to = scores + (int64_t)row * a.max_pages + base + x * step;
-          *to = g0 == 0 ? best : nanmax(*to, best);
-        }
+        const float t = warp_sums4(s);
+        const bool real = g0 + 4 * c + lane / 8 < G;
+        nan[x] |= real && t != t;
+        best[x] = max(best[x], real ? score_key(t) : 0u);
       }
     }
+  }
+#pragma unroll
+  for (int x = 0; x < kScorePages; ++x) {
+    if (x >= n) break;
+    uint32_t key = __reduce_max_sync(0xffffffffu, best[x]);
+    if (__any_sync(0xffffffffu, nan[x])) key = kNanKey;
+    if (lane == 0) keys[(int64_t)row * a.max_pages + j0 + x] = key;
   }
 }
 
 // One CTA per (request, key head): the key of the top-th best page by four
 // passes over 8 bits of the keys, then the pages above it and the lowest pages
 // at it, in ascending order.
-__global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a, const float* __restrict__ scores) {
+__global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a,
+                                                              const uint32_t* __restrict__ row_keys) {
   __shared__ int hist[256];
   __shared__ int sh_bin, sh_left;
   __shared__ int wsum[2][kTopThreads / 32];
@@ -147,9 +169,9 @@ __global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a, con
     for (int i = threadIdx.x; i < a.top; i += kTopThreads) out[i] = i < pages ? i : -1;
     return;
   }
-  const float* s = scores + (int64_t)row * a.max_pages;
+  const uint32_t* s = row_keys + (int64_t)row * a.max_pages;
   auto make_key = [&](int j) -> uint32_t {
-    return (j < a.keep_first || j >= pages - a.keep_last) ? 0xffffffffu : score_key(s[j]);
+    return (j < a.keep_first || j >= pages - a.keep_last) ? 0xffffffffu : s[j];
   };
   for (int j = threadIdx.x; j < min(pages, kTopKeys); j += kTopThreads) keys[j] = make_key(j);
   auto key_of = [&](int j) -> uint32_t { return j < kTopKeys ? keys[j] : make_key(j); };
@@ -217,21 +239,23 @@ size_t kv4_select_workspace(const SagaKv4Args& a) {
 }
 
 int launch_kv4_select(const SagaKv4Args& a, cudaStream_t st) {
-  float* scores = reinterpret_cast<float*>(a.workspace);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(a.workspace);
   const int rows = a.B * a.pool.Hk;
   const int G = a.Hq / a.pool.Hk;
   if (rows > 65535) return abi_fail(SAGA_ERR_UNSUPPORTED, "more than 65535 (request, key head) rows");
   if (a.max_pages > a.top) {
-    // a page per warp until every SM has eight CTAs
-    const int want = (a.max_pages + 7) / 8, most = std::max(1, 8 * 148 / rows);
-    const dim3 grid(std::min(want, most), rows);
+    // one page per warp where the SMs hold that many warps (two CTAs of eight each), else up to four
+    const int64_t warps = (int64_t)rows * a.max_pages;
+    const int per_warp = (int)std::min<int64_t>(kScorePages, (warps + 16 * 148 - 1) / (16 * 148));
+    const dim3 grid((a.max_pages + 8 * per_warp - 1) / (8 * per_warp), rows);
     auto go = [&](auto* t, auto d) {
       using T = std::remove_pointer_t<decltype(t)>;
       return kv4_launch("kv4_score_kernel",
-                        G <= 4   ? kv4_score_kernel<T, d.value, 4>
-                        : G <= 8 ? kv4_score_kernel<T, d.value, 8>
-                                 : kv4_score_kernel<T, d.value, 16>,
-                        grid, 256, 0, st, a, scores);
+                        G <= 4    ? kv4_score_kernel<T, d.value, 1>
+                        : G <= 8  ? kv4_score_kernel<T, d.value, 2>
+                        : G <= 12 ? kv4_score_kernel<T, d.value, 3>
+                                  : kv4_score_kernel<T, d.value, 4>,
+                        grid, 256, 0, st, a, keys, per_warp);
     };
     auto by_d = [&](auto* t) {
       return a.pool.D == 128 ? go(t, std::integral_constant<int, 128>()) : go(t, std::integral_constant<int, 64>());
@@ -241,7 +265,7 @@ int launch_kv4_select(const SagaKv4Args& a, cudaStream_t st) {
                                           : by_d((float*)nullptr);
     if (rc) return rc;
   }
-  return kv4_launch("kv4_top_kernel", kv4_top_kernel, dim3(rows), kTopThreads, 0, st, a, scores);
+  return kv4_launch("kv4_top_kernel", kv4_top_kernel, dim3(rows), kTopThreads, 0, st, a, keys);
 }
 
 }  // namespace saga

@@ -17,12 +17,13 @@ struct TableRow {
   int held;   // pages held before the step
 };
 
-// Exclusive sums over the CTA's threads of three values; totals in tot.
-__device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], long long (*sm)[33]) {
+// Exclusive sums over the CTA's threads of N values; totals in tot.
+template <int N>
+__device__ __forceinline__ void scan(long long (&v)[N], long long (&tot)[N], long long (*sm)[33]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long inc[3];
+  long long inc[N];
 #pragma unroll
-  for (int j = 0; j < 3; ++j) {
+  for (int j = 0; j < N; ++j) {
     long long x = v[j];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -33,7 +34,7 @@ __device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], lo
     if (lane == 31) sm[j][warp] = x;
   }
   __syncthreads();
-  if (warp < 3) {
+  if (warp < N) {
     const long long own = sm[warp][lane];
     long long x = own;
 #pragma unroll
@@ -47,7 +48,7 @@ __device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], lo
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 3; ++j) {
+  for (int j = 0; j < N; ++j) {
     tot[j] = sm[j][32];
     v[j] = sm[j][warp] + inc[j] - v[j];
   }
@@ -55,13 +56,15 @@ __device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], lo
 }
 
 __device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
-  __shared__ long long sm[3][33];
+  __shared__ long long sm[2][33];
+  __shared__ int taken_sm;
+  if (threadIdx.x == 0) taken_sm = 0;
   const int shift = __ffs(a.page_len) - 1;
   const long long cover = (long long)a.max_pages << shift;
   const int head = a.free_state[0];
   const int count = min(max(a.free_state[1], 0), a.ring);
   const int h0 = a.ring ? (int)((unsigned)max(head, 0) % (unsigned)a.ring) : 0;
-  long long tok = 0, want = 0, ret = 0, taken = 0;
+  long long tok = 0, want = 0, ret = 0;
   for (int base = 0; base < a.B; base += kScan) {
     const int b = base + threadIdx.x;
     const bool in = b < a.B;
@@ -70,26 +73,22 @@ __device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
     const int add = max(raw, 0);
     const long long end = (long long)len + add;
     const int held = (int)(((long long)len + a.page_len - 1) >> shift);
-    long long v[3] = {add, 0, 0}, tot[3];
-    scan3(v, tot, sm);
-    const long long start = tok + v[0];
-    tok += tot[0];
+    long long v1[1] = {add}, tot1[1];
+    scan(v1, tot1, sm);
+    const long long start = tok + v1[0];
+    tok += tot1[0];
     const bool fits = end <= cover && start + add <= a.num_tokens;
     const int need = fits ? (int)(((end + a.page_len - 1) >> shift) - held) : 0;
     const int back = in && raw < 0 && a.ring ? min(held, a.max_pages) : 0;
-    v[0] = 0;
-    v[1] = need;
-    v[2] = back;
-    scan3(v, tot, sm);
-    const long long upto = want + v[1] + need;
+    long long v[2] = {need, back}, tot[2];
+    scan(v, tot, sm);
+    const long long upto = want + v[0] + need;
     const bool granted = fits && (need == 0 || upto <= count);
-    const long long before = ret + v[2];
-    want += tot[1];
-    ret += tot[2];
-    v[0] = granted ? need : 0;
-    v[1] = v[2] = 0;
-    scan3(v, tot, sm);
-    taken += tot[0];
+    const long long before = ret + v[1];
+    want += tot[0];
+    ret += tot[1];
+    // the granted requests that need pages are the first ones that do, so the last one's sum is the total
+    if (granted && need) atomicMax(&taken_sm, (int)upto);
     if (in) {
       TableRow r;
       r.len = granted ? len : -1;
@@ -102,28 +101,46 @@ __device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
       if (!granted && add > 0) set_status(a.status, SAGA_STATUS_OUT_OF_PAGES);
     }
   }
+  __syncthreads();
   if (threadIdx.x == 0) {
+    const int taken = taken_sm;
     a.offsets[0] = 0;
     a.free_state_out[0] = a.ring ? (int)((h0 + taken) % a.ring) : 0;
     a.free_state_out[1] = (int)(count - taken + ret);
   }
 }
 
-// Token `i`: its request by bisection of the offsets, its slot and position;
-// the first token of a new page also writes the page table's entry.
-__device__ __forceinline__ void table_token(const SagaPageTableArgs& a, const TableRow* rows, int64_t i) {
-  int lo = 0, hi = a.B;  // offsets[lo] <= i; hi: first request that begins after i
+constexpr int kShared = 2048;  // offsets kept in shared memory (a bisection in global memory waits at every step)
+
+// Copies the offsets to shared memory if they fit; returns where to read them.
+__device__ __forceinline__ const int32_t* stage_offsets(const int32_t* offsets, int B, int32_t* sm) {
+  if (B >= kShared) return offsets;
+  for (int i = threadIdx.x; i <= B; i += blockDim.x) sm[i] = offsets[i];
+  __syncthreads();
+  return sm;
+}
+// The request that row i belongs to: offsets[lo] <= i < offsets[lo + 1].
+__device__ __forceinline__ int find_request(const int32_t* offsets, int B, int64_t i) {
+  int lo = 0, hi = B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a.offsets[mid] <= i) lo = mid;
+    if (offsets[mid] <= i) lo = mid;
     else hi = mid;
   }
+  return lo;
+}
+
+// Token `i`: its request, slot and position; the first token of a new page also
+// writes the page table's entry.
+__device__ __forceinline__ void table_token(const SagaPageTableArgs& a, const TableRow* rows, const int32_t* offsets,
+                                            int64_t i) {
   int64_t slot = -1;
   int pos = 0;
-  if (a.B > 0 && i < a.offsets[a.B]) {
+  if (a.B > 0 && i < offsets[a.B]) {
+    const int lo = find_request(offsets, a.B, i);
     const TableRow r = rows[lo];
     if (r.len >= 0) {
-      pos = r.len + (int)(i - a.offsets[lo]);
+      pos = r.len + (int)(i - offsets[lo]);
       const int shift = __ffs(a.page_len) - 1;
       const int p = pos >> shift, off = pos & (a.page_len - 1);
       int32_t* entry = a.page_table + (int64_t)lo * a.pt_sb + p;
@@ -154,22 +171,26 @@ __global__ void __launch_bounds__(kScan) page_tables_scan_kernel(SagaPageTableAr
   TableRow* rows = reinterpret_cast<TableRow*>(a.workspace);
   table_scan(a, rows);
   if (!all) return;
+  __shared__ int32_t off_sm[kShared + 1];
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < a.num_tokens; i += kScan) table_token(a, rows, i);
+  const int32_t* offsets = stage_offsets(a.offsets, a.B, off_sm);
+  for (int64_t i = threadIdx.x; i < a.num_tokens; i += kScan) table_token(a, rows, offsets, i);
   for (int b = threadIdx.x >> 5; b < a.B; b += kScan / 32) table_return(a, rows, b);
 }
 
 __global__ void __launch_bounds__(256) page_tables_token_kernel(SagaPageTableArgs a) {
   pdl_wait();
   const TableRow* rows = reinterpret_cast<const TableRow*>(a.workspace);
+  __shared__ int32_t off_sm[kShared + 1];
+  const int32_t* offsets = stage_offsets(a.offsets, a.B, off_sm);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < a.num_tokens) table_token(a, rows, i);
+  if (i < a.num_tokens) table_token(a, rows, offsets, i);
   for (int b = (int)(i >> 5); b < a.B; b += (int)gridDim.x * 8) table_return(a, rows, b);
 }
 
 __global__ void __launch_bounds__(kScan) slot_offsets_kernel(int B, int64_t cover, const int32_t* starts,
                                                              const int32_t* lens, int32_t* offsets, int* status) {
-  __shared__ long long sm[3][33];
+  __shared__ long long sm[1][33];
   pdl_wait();
   long long tok = 0;
   for (int base = 0; base < B; base += kScan) {
@@ -183,8 +204,8 @@ __global__ void __launch_bounds__(kScan) slot_offsets_kernel(int B, int64_t cove
       }
       n = max(end - max(starts ? starts[b] : 0, 0), 0ll);
     }
-    long long v[3] = {n, 0, 0}, tot[3];
-    scan3(v, tot, sm);
+    long long v[1] = {n}, tot[1];
+    scan(v, tot, sm);
     if (b < B) offsets[b + 1] = (int)min(tok + v[0] + n, 0x7fffffffll);
     tok += tot[0];
   }
@@ -195,16 +216,13 @@ __global__ void __launch_bounds__(256) slot_map_kernel(int B, int page_len, cons
                                                        const int32_t* starts, int64_t T_, int64_t* slots,
                                                        const int32_t* offsets) {
   pdl_wait();
+  __shared__ int32_t off_sm[kShared + 1];
+  offsets = stage_offsets(offsets, B, off_sm);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= T_) return;
   int64_t slot = -1;
   if (B > 0 && i < offsets[B]) {
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (offsets[mid] <= i) lo = mid;
-      else hi = mid;
-    }
+    const int lo = find_request(offsets, B, i);
     const int pos = max(starts ? starts[lo] : 0, 0) + (int)(i - offsets[lo]);
     const int shift = __ffs(page_len) - 1;
     slot = (int64_t)pt[(int64_t)lo * pt_sb + (pos >> shift)] * page_len + (pos & (page_len - 1));

@@ -487,6 +487,22 @@ def test_select_ties_go_to_the_lower_page_and_nan_is_last():
     assert blocks[0, 0].tolist() == [0, 1, 2, 3, 39]
 
 
+def test_pages_of_nan_keys_are_selected_last():
+    from saga_b200 import kv4
+    d, pl = 64, 32
+    c = Cache([10 * pl], 1, 1, d, pl, seed=27, bounds=True)
+    for p in (4, 6):
+        k = torch.full((pl, 1, d), float("nan"), dtype=torch.bfloat16, device=DEV)
+        kv4.kv4_write(c.pool, k, k, slots_of(c.table, 0, (p + 1) * pl, pl, p * pl))
+        assert torch.isnan(c.pool.k_lo[int(c.table[0, p])].float()).all()
+        assert torch.isnan(c.pool.k_hi[int(c.table[0, p])].float()).all()
+    q = torch.randn((1, 3, 1, d), generator=gen(28), device=DEV).to(torch.bfloat16)
+    blocks, _ = kv4.kv4_select(q, c.pool, c.table, c.device_lens, 8)
+    assert blocks[0, 0].tolist() == [0, 1, 2, 3, 5, 7, 8, 9]
+    blocks, _ = kv4.kv4_select(q, c.pool, c.table, c.device_lens, 9)
+    assert blocks[0, 0].tolist() == [0, 1, 2, 3, 4, 5, 7, 8, 9]
+
+
 def test_select_more_pages_than_fit_shared_memory():
     from saga_b200 import kv4
     d, pl, n, top = 64, 32, 9000, 50
