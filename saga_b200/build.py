@@ -3,7 +3,10 @@
     python -m saga_b200.build [--force]
 
 Sources: saga_b200/csrc/*.cu. Output: saga_b200/libsaga_b200.so. The library
-links the CUDA runtime statically and has no PyTorch dependency.
+links the CUDA runtime statically and has no PyTorch dependency. The host calls
+of the 4-bit cache operators (saga_b200/csrc/fastcall.cpp) are a CPython module
+of their own, saga_b200/_fastcall.so, which knows torch and is bound to the
+library at run time.
 """
 from __future__ import annotations
 
@@ -20,6 +23,8 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsaga_b200.so")
 STAMP = os.path.join(HERE, ".libsaga_b200.stamp")
+FAST_SRC = os.path.join(CSRC, "fastcall.cpp")
+FAST = os.path.join(HERE, "_fastcall.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -44,7 +49,7 @@ def _sources():
 def _digest() -> str:
     h = hashlib.sha256()
     files = _sources() + sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")))
-    files.append(os.path.join(REPO, "include", "saga_b200.h"))
+    files += [FAST_SRC, os.path.join(REPO, "include", "saga_b200.h")]
     for f in files:
         with open(f, "rb") as fh:
             h.update(os.path.basename(f).encode())
@@ -54,10 +59,28 @@ def _digest() -> str:
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(STAMP):
+    if not os.path.exists(LIB) or not os.path.exists(FAST) or not os.path.exists(STAMP):
         return False
     with open(STAMP) as f:
         return f.read().strip() == _digest()
+
+
+def _fast_command(out: str) -> list:
+    """The g++ command of the torch-facing call module."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(os.path.dirname(_nvcc()), "..", "include")]
+    for d in include_paths():
+        cmd += ["-isystem", d]
+    cmd += [FAST_SRC, "-o", out]
+    for d in library_paths():
+        cmd += ["-L", d]
+    return cmd + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -74,6 +97,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         objs.append(obj)
         cmd = [nvcc, *ARCH, *FLAGS, "-I", os.path.join(REPO, "include"), "-dc" if False else "-c", src, "-o", obj]
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    fast_tmp = FAST + ".tmp"
+    procs.append((FAST_SRC, subprocess.Popen(_fast_command(fast_tmp), stdout=subprocess.PIPE,
+                                             stderr=subprocess.STDOUT, text=True)))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -90,6 +116,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         sys.stdout.write(r.stdout + r.stderr)
         raise RuntimeError("link failed")
     os.replace(tmp, LIB)
+    os.replace(fast_tmp, FAST)
     with open(STAMP, "w") as f:
         f.write(_digest())
     return LIB

@@ -26,23 +26,18 @@ import torch
 from . import _lib as L
 from .ops import _DT, _STATUS, status_tensor
 
+try:
+    from . import _fastcall as _fast  # after torch, whose libraries it uses
+except ImportError as e:
+    raise ImportError("saga_b200/_fastcall.so is missing or does not load: build it with "
+                      "`python -m saga_b200.build`") from e
+_fast.bind(*(ctypes.cast(getattr(L.lib, f), ctypes.c_void_p).value for f in
+             ("saga_kv4_write", "saga_kv4_read", "saga_kv4_workspace_bytes", "saga_kv4_decode", "saga_kv4_select",
+              "saga_page_tables")))
+
 GROUP = 64  # values that share a scale
-_SCRATCH: dict = {}
 _I32, _I64 = torch.int32, torch.int64
 _raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _scratch(index: int, stream: int, nbytes: int) -> int:
-    """Address of ``nbytes`` of workspace for calls on this stream. The kernels
-    do not care what it holds. Smaller ones are kept, since a CUDA graph may
-    refer to them."""
-    have = _SCRATCH.get((index, stream))
-    if have is None or have[-1].numel() < nbytes:
-        grown = torch.empty(max(nbytes, 2 * have[-1].numel() if have else 1 << 20), dtype=torch.uint8,
-                            device=torch.device("cuda", index))
-        have = _SCRATCH.setdefault((index, stream), [])
-        have.append(grown)
-    return have[-1].data_ptr()
 
 
 def _status(index: int) -> int:
@@ -148,8 +143,8 @@ class Kv4Pool:
         self._index = self.device.index
         self._desc = self.descriptor()
         self._ref = ctypes.byref(self._desc)
-        self._status = status_tensor(self.device).data_ptr()
-        self._sizes: dict = {}  # workspace bytes per op and shapes
+        self._status = _status(self._index)
+        self._handle = _fast.pool(ctypes.addressof(self._desc), self._index, self._status)
 
     def descriptor(self) -> L.SagaKv4Pool:
         """The C descriptor of the pool's tensors."""
@@ -196,6 +191,8 @@ def kv4_write(pool: Kv4Pool, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
     last slot is written gets its key bounds. Two rows must not name one slot."""
     if torch.compiler.is_compiling():
         return torch.ops.saga.kv4_write(*_tensors(pool), k, v, slots)
+    if _fast.write(pool._handle, k, v, slots):
+        return
     T = _rows(pool, k, v, slots)
     ks, vs = k.stride(), v.stride()
     with _on_device(pool._index):
@@ -212,6 +209,9 @@ def kv4_read(pool: Kv4Pool, slots: torch.Tensor, dtype: torch.dtype = torch.bflo
     outside the pool). E.g. the history that a prompt chunk attends to."""
     if torch.compiler.is_compiling():
         return torch.ops.saga.kv4_read(*_tensors(pool), slots, dtype)
+    got = _fast.read(pool._handle, slots, dtype)
+    if got is not None:
+        return got
     T = slots.numel()
     code = _dtype_code(dtype)
     at = _ints("slots", slots, pool._index, _I64, (T,))
@@ -273,15 +273,11 @@ def _kv4_run(fn, name: str, a: L.SagaKv4Args, op: int, pool: Kv4Pool) -> None:
     index = pool._index
     with _on_device(index):
         ref = ctypes.byref(a)
-        key = (op, a.dtype, a.B, a.Hq, a.max_pages, a.top)
-        nbytes = pool._sizes.get(key)
-        if nbytes is None:
-            nbytes = L.lib.saga_kv4_workspace_bytes(ref, op)
-            if nbytes == 0:
-                raise L.SagaError(L.SAGA_ERR_INVALID, "saga_kv4_workspace_bytes")
-            pool._sizes[key] = nbytes
+        nbytes = L.lib.saga_kv4_workspace_bytes(ref, op)
+        if nbytes == 0:
+            raise L.SagaError(L.SAGA_ERR_INVALID, "saga_kv4_workspace_bytes")
         stream = _raw_stream(index)
-        a.workspace = _scratch(index, stream, nbytes)
+        a.workspace = _fast.scratch(index, stream, nbytes)
         a.workspace_bytes = nbytes
         rc = fn(ref, stream)
     if rc:
@@ -301,6 +297,9 @@ def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     """
     if torch.compiler.is_compiling():
         return torch.ops.saga.kv4_decode(*_tensors(pool), query, page_table, lens, scaling, starts, blocks, counts)
+    out = _fast.decode(pool._handle, query, page_table, lens, scaling, starts, blocks, counts)
+    if out is not None:
+        return out
     a = _kv4_args(query, pool, page_table, lens)
     B, Hq, D = a.B, a.Hq, pool.head_dim
     a.scaling = D ** -0.5 if scaling is None else float(scaling)
@@ -339,6 +338,10 @@ def kv4_select(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     """
     if torch.compiler.is_compiling():
         return torch.ops.saga.kv4_select(*_tensors(pool), query, page_table, lens, top, keep_first, keep_last)
+    if pool.k_lo is not None:
+        got = _fast.select(pool._handle, query, page_table, lens, top, keep_first, keep_last)
+        if got is not None:
+            return got
     a = _kv4_args(query, pool, page_table, lens)
     if pool.k_lo is None:
         raise ValueError("kv4_select needs a pool with bounds=True")
@@ -392,6 +395,10 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
         return step
     if not page_table.is_cuda:
         _bad_cuda()
+    got = _fast.tables(page_table, lens, new_lens, free_pages, free_state, num_tokens, page_len, lens_out,
+                       free_state_out, _status(page_table.get_device()))
+    if got is not None:
+        return PageStep._make(got)
     index, dev = page_table.get_device(), page_table.device
     B, ring = lens.numel(), free_pages.numel()
     num_tokens = int(num_tokens)
@@ -423,7 +430,7 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     nbytes = max(16 * B, 16)
     with _on_device(index):
         stream = _raw_stream(index)
-        a.workspace = _scratch(index, stream, nbytes)
+        a.workspace = _fast.scratch(index, stream, nbytes)
         a.workspace_bytes = nbytes
         rc = L.lib.saga_page_tables(ctypes.byref(a), stream)
     if rc:
