@@ -251,11 +251,12 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
 
 // Bounds of the pages whose last slot is among the slots: a CTA looks at
 // `strip` tokens and takes the bounds of the pages that they complete. Threads
-// split a page into D/8 words of a row by 8 (16) rows.
+// split a page into D/8 words of a row by 16 (32) rows.
+constexpr int kBoundThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t T_, int strip,
+__global__ void __launch_bounds__(kBoundThreads) kv4_bounds_kernel(SagaKv4Pool p, int64_t T_, int strip,
                                                          const int64_t* __restrict__ slots) {
-  constexpr int W = D / 8, ROWS = 128 / W;
+  constexpr int W = D / 8, ROWS = kBoundThreads / W;
   __shared__ float red[2][ROWS][D];
   pdl_wait();
   __shared__ int64_t done[32];
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(128) kv4_bounds_kernel(SagaKv4Pool p, int64_t 
         lo[i] = INFINITY;
         hi[i] = -INFINITY;
       }
-#pragma unroll 4
+#pragma unroll 8
       for (int off = rr; off < p.page_len; off += ROWS) {
         const uint8_t* tile =
             reinterpret_cast<const uint8_t*>(p.k) + kv4_tile_at<D>(page, h, p.Hk, off, p.page_len);
@@ -382,8 +383,8 @@ int launch_kv4_write(const SagaKv4Pool& p, int dt, int64_t T, const void* k, int
   // one token per CTA where every token may complete a page; runs of prompt tokens complete one in 32 at most
   const int strip = T <= 4096 ? 1 : 32;
   const unsigned nb = (unsigned)((T + strip - 1) / strip);
-  return kv4_launch("kv4_bounds_kernel", p.D == 128 ? kv4_bounds_kernel<128> : kv4_bounds_kernel<64>, dim3(nb), 128, 0,
-                    st, p, T, strip, slots);
+  return kv4_launch("kv4_bounds_kernel", p.D == 128 ? kv4_bounds_kernel<128> : kv4_bounds_kernel<64>, dim3(nb),
+                    kBoundThreads, 0, st, p, T, strip, slots);
 }
 
 int launch_kv4_read(const SagaKv4Pool& p, int dt, int64_t T, const int64_t* slots, void* k, int64_t k_st,

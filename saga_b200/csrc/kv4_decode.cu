@@ -41,8 +41,8 @@ constexpr int kMinTiles = 4;        // tiles of a CTA's run, at least: one warp 
 constexpr int kRingBytes = 216 * 1024;  // of all warps; static shared memory has the rest
 constexpr float kHead = 12.f;     // log2 of the greatest weight where the stabiliser was last set
 constexpr float kLow = 2048.f;    // SPLIT: the second term of a weight is held this much greater
-// -15 and -16 * 15 in units of 2^-24, twice
-constexpr uint32_t kMinus15 = 0x800f800fu, kMinus240 = 0x80f080f0u;
+// -15, -16 * 15 and their sum in units of 2^-24, twice
+constexpr uint32_t kMinus15 = 0x800f800fu, kMinus240 = 0x80f080f0u, kMinus255 = 0x80ff80ffu;
 constexpr float kNegInf = -INFINITY;
 
 // Query heads of a key head are cut into slot groups: consecutive heads, at most
@@ -110,6 +110,15 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The same with nothing added: the accumulators need not be cleared first.
+__device__ __forceinline__ void mma16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, "
+      "%10, %10};\n"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 // log2 of a positive bfloat16 scale, within 0.09 (its bits are a piecewise
 // linear logarithm). It only places the stabiliser of the weights.
 __device__ __forceinline__ float rough_log2(uint32_t bf16_bits) {
@@ -158,8 +167,13 @@ __device__ __forceinline__ RowInfo row_info(const SagaKv4Args& a, int r) {
   return i;
 }
 
+// Quotient of numbers that are not negative; 32 bits where they fit, since a 64-bit division takes about a
+// hundred instructions.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 __device__ __forceinline__ long long tiles_per_cta(long long total, int grid) {
-  return max((total + grid - 1) / grid, (long long)kMinTiles);
+  return max(divide(total + grid - 1, grid), (long long)kMinTiles);
 }
 
 // D: head_dim; NT: tiles of eight slots; SPLIT: queries and weights as two fp16
@@ -169,6 +183,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   constexpr int NG = D / 64, CH = D / 32, NP = SPLIT ? 2 : 1, SLOTS = 8 * NT;
   constexpr int TB = kv4_tile_bytes(D);
   constexpr int META = kKv4Tile * (D / 2);
+  // Whether channel rows 0-7 of a product take both codes of a byte, c + 16 c' (rows 8-15 have 16 c' and are
+  // taken off at the end): an AND less per code, four bits less of the sums.
+  constexpr bool kPairs = !SPLIT;
   constexpr int RP = D + 4;   // pitch of a warp's outputs when the warps meet
   constexpr int QP = D + 8;   // pitch of the queries
   constexpr int QT = 16, QC = D / QT;  // threads per slot's query, channels of each
@@ -507,10 +524,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
           // consecutive products go to different accumulators: one chain waits for itself at every step
           float acc[4][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) acc[j][x] = 0.f;
-#pragma unroll
           for (int ch = c0; ch < c0 + STEP; ++ch)
 #pragma unroll
             for (int t = 0; t < NP; ++t) {
@@ -528,8 +541,10 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const uint32_t w = h ? kreg[j][ch] >> 8 : kreg[j][ch];
-                  mma16(acc[j], q[0][2 * h], NT == 2 ? q[NT - 1][2 * h] : 0u, q[0][2 * h + 1],
-                        NT == 2 ? q[NT - 1][2 * h + 1] : 0u, w & 0x000f000fu, w & 0x00f000f0u);
+                  const uint32_t x0 = w & 0x000f000fu, x1 = w & 0x00f000f0u;
+                  const uint32_t a1 = NT == 2 ? q[NT - 1][2 * h] : 0u, a3 = NT == 2 ? q[NT - 1][2 * h + 1] : 0u;
+                  if (ch == c0 && t == 0 && h == 0) mma16_first(acc[j], q[0][2 * h], a1, q[0][2 * h + 1], a3, x0, x1);
+                  else mma16(acc[j], q[0][2 * h], a1, q[0][2 * h + 1], a3, x0, x1);
                 }
             }
 #pragma unroll
@@ -673,22 +688,20 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
             // products y = 2x + m: chunk 2g + x (positions 0-7 in t[2x], 8-15 in t[2x + 1]), bytes m and m + 2
             float s[NP][4][4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                s[0][y][x] = s[NP - 1][y][x] = 0.f;
-              }
-#pragma unroll
             for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
               for (int n = 0; n < NP; ++n)
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                  const uint32_t w0 = t[g][jj][y & 2] >> (8 * (y & 1)), w1 = t[g][jj][(y & 2) + 1] >> (8 * (y & 1));
-                  const uint32_t e0 = w0 & 0x000f000fu, h0 = w0 & 0x00f000f0u, e1 = w1 & 0x000f000fu,
-                                 h1 = w1 & 0x00f000f0u;
-                  mma16(s[n][y], centre(e0, kMinus15), centre(h0, kMinus240), centre(e1, kMinus15),
-                        centre(h1, kMinus240), wv[g][jj][n][0], wv[g][jj][n][1]);
+                  const uint32_t w0 = t[g][jj][y & 2], w1 = t[g][jj][(y & 2) + 1];
+                  // bytes y & 1 and 2 + (y & 1) as fp16: c + 16 c' of two positions
+                  const uint32_t u0 = y & 1 ? __byte_perm(w0, 0, 0x4341) : w0 & 0x00ff00ffu;
+                  const uint32_t u1 = y & 1 ? __byte_perm(w1, 0, 0x4341) : w1 & 0x00ff00ffu;
+                  const uint32_t a0 = centre(kPairs ? u0 : u0 & 0x000f000fu, kPairs ? kMinus255 : kMinus15),
+                                 a2 = centre(kPairs ? u1 : u1 & 0x000f000fu, kPairs ? kMinus255 : kMinus15),
+                                 a1 = centre(u0 & 0x00f000f0u, kMinus240), a3 = centre(u1 & 0x00f000f0u, kMinus240);
+                  if (jj == 0) mma16_first(s[n][y], a0, a1, a2, a3, wv[g][jj][n][0], wv[g][jj][n][1]);
+                  else mma16(s[n][y], a0, a1, a2, a3, wv[g][jj][n][0], wv[g][jj][n][1]);
                 }
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
@@ -737,11 +750,15 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       if (mine > 0) {
 #pragma unroll
         for (int m = 0; m < D / 16; ++m) {
-          // rows r8: channel d; rows r8 + 8: 16 times channel d + 1
+          // rows r8: channel d (kPairs: plus 16 times channel d + 1); rows r8 + 8: 16 times channel d + 1
           const int d = 32 * (m / 2) + 4 * r8 + 2 * (m & 1);
           float e0, e1, h0, h1;
           unpack2(o[i][m][0], e0, e1);
           unpack2(o[i][m][1], h0, h1);
+          if constexpr (kPairs) {
+            e0 -= h0;
+            e1 -= h1;
+          }
           float* s0 = so + (8 * i + 2 * c4) * RP + d;
           *reinterpret_cast<float2*>(s0) =
               make_float2(fmaf(e0, 0x1p23f, z0[m / 4]), fmaf(h0, 0x1p19f, z0[m / 4]));
@@ -807,15 +824,13 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
 
 // Joins the partial results of items that CTA borders cut, and writes the zeros
 // of rows without positions. One CTA per (request, query head): a warp takes
-// every kJoinWarps-th part, a lane four channels.
-constexpr int kJoinWarps = 8;
-constexpr int kJoinThreads = 32 * kJoinWarps;
-template <int D>
-__global__ void __launch_bounds__(kJoinThreads) kv4_combine_kernel(const DecodePlan4 p, int grid, int slots) {
+// every WARPS-th part, a lane four channels.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) kv4_combine_kernel(const DecodePlan4 p, int grid, int slots) {
   constexpr int LPD = D / 4;            // lanes of a part
   constexpr int PPW = 32 / LPD;         // parts that a warp reads at a time
-  __shared__ float sm_m[kJoinWarps], sm_l[kJoinWarps];
-  __shared__ __align__(16) float sm_o[kJoinWarps * PPW][D];
+  __shared__ float sm_m[WARPS], sm_l[WARPS];
+  __shared__ __align__(16) float sm_o[WARPS * PPW][D];
   const SagaKv4Args& a = p.a;
   const int b = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -827,52 +842,65 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_combine_kernel(const DecodeP
   pdl_wait();
   if (threadIdx.x == 0 && a.lens[b] > a.max_pages * a.pool.page_len) set_status(a.status, SAGA_STATUS_PAGE_RANGE);
   const long long total = p.prefix[a.B * a.pool.Hk], first = p.prefix[row];
-  const long long tiles = (p.prefix[row + 1] - first) / p.groups;
+  const long long tiles = divide(p.prefix[row + 1] - first, p.groups);
   const int64_t at = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
   if (tiles == 0) {
-    if (threadIdx.x < D) store_out(a.out, a.dtype, at + threadIdx.x, 0.f);
+    for (int c = threadIdx.x; c < D; c += 32 * WARPS) store_out(a.out, a.dtype, at + c, 0.f);
     return;
   }
   const long long per = tiles_per_cta(total, grid);
   const long long begin = first + sg * tiles, end = begin + tiles;
-  const int c0 = (int)(begin / per), n = (int)((end - 1) / per) - c0 + 1;
+  const int c0 = (int)divide(begin, per), n = (int)divide(end - 1, per) - c0 + 1;
   if (n == 1) return;  // one CTA had the whole item
   // part i: of CTA c0 + i; only the first part can begin with the item
   auto record = [&](int i) { return ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * slots + (h - grp.h0); };
+  const int sub = lane / LPD, d = (lane % LPD) * 4;
+  // the first parts of each warp are on their way while the maximum is found
+  constexpr int kEarly = 4;
+  float4 early[kEarly];
+#pragma unroll
+  for (int j = 0; j < kEarly; ++j) {
+    const int i = (warp + j * WARPS) * PPW + sub;
+    if (i < n) early[j] = *reinterpret_cast<const float4*>(p.part_o + record(i) * D + d);
+  }
   float m = kNegInf;
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) m = fmaxf(m, p.part_ml[record(i) * 2]);
+  for (int i = threadIdx.x; i < n; i += 32 * WARPS) m = fmaxf(m, p.part_ml[record(i) * 2]);
   m = warp_max(m);
   if (lane == 0) sm_m[warp] = m;
   __syncthreads();
   float M = sm_m[0];
 #pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w) M = fmaxf(M, sm_m[w]);
-  const int sub = lane / LPD, d = (lane % LPD) * 4;
+  for (int w = 1; w < WARPS; ++w) M = fmaxf(M, sm_m[w]);
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   float L = 0.f;
-#pragma unroll 4
-  for (int i = warp * PPW + sub; i < n; i += kJoinWarps * PPW) {
-    const int64_t rec = record(i);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + rec * 2);
-    const float4 t = *reinterpret_cast<const float4*>(p.part_o + rec * D + d);
+  auto add = [&](int i, const float4& t) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + record(i) * 2);
     const float f = ml.x == kNegInf ? 0.f : ex2(ml.x - M);
     L = fmaf(ml.y, f, L);
     O.x = fmaf(t.x, f, O.x);
     O.y = fmaf(t.y, f, O.y);
     O.z = fmaf(t.z, f, O.z);
     O.w = fmaf(t.w, f, O.w);
+  };
+#pragma unroll
+  for (int j = 0; j < kEarly; ++j) {
+    const int i = (warp + j * WARPS) * PPW + sub;
+    if (i < n) add(i, early[j]);
   }
+#pragma unroll 4
+  for (int i = (warp + kEarly * WARPS) * PPW + sub; i < n; i += WARPS * PPW)
+    add(i, *reinterpret_cast<const float4*>(p.part_o + record(i) * D + d));
   *reinterpret_cast<float4*>(&sm_o[warp * PPW + sub][d]) = O;
   if (PPW == 2) L += __shfl_xor_sync(0xffffffffu, L, 16);
   if (lane == 0) sm_l[warp] = L;
   __syncthreads();
-  if (threadIdx.x < D) {
+  for (int c = threadIdx.x; c < D; c += 32 * WARPS) {
     float o = 0.f, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) l += sm_l[w];
+    for (int w = 0; w < WARPS; ++w) l += sm_l[w];
 #pragma unroll
-    for (int w = 0; w < kJoinWarps * PPW; ++w) o += sm_o[w][threadIdx.x];
-    store_out(a.out, a.dtype, at + threadIdx.x, l == 0.f ? 0.f : o / l);
+    for (int w = 0; w < WARPS * PPW; ++w) o += sm_o[w][c];
+    store_out(a.out, a.dtype, at + c, l == 0.f ? 0.f : o / l);
   }
 }
 
@@ -943,8 +971,13 @@ int launch(const DecodePlan4& p, const DecodeSizes& z, cudaStream_t st) {
     raised = kRingBytes;
   }
   if (int rc = kv4_launch("kv4_decode_kernel", fn, dim3(z.grid), kDecThreads, smem, st, p)) return rc;
-  return kv4_launch("kv4_combine_kernel", kv4_combine_kernel<D>, dim3((unsigned)(p.a.B * p.a.Hq)), kJoinThreads, 0, st,
-                    p, z.grid, z.slots);
+  // few rows have many parts each (147 parts: 6.1 us with 16 warps, 7.5 us with 8); many rows have few, and
+  // their CTAs' number counts (768 rows: 6.7 us with 8 warps, 12.5 us with 16)
+  const int rows = p.a.B * p.a.Hq;
+  return rows <= z.grid ? kv4_launch("kv4_combine_kernel", kv4_combine_kernel<D, 16>, dim3((unsigned)rows), 512, 0, st,
+                                     p, z.grid, z.slots)
+                        : kv4_launch("kv4_combine_kernel", kv4_combine_kernel<D, 4>, dim3((unsigned)rows), 128, 0, st,
+                                     p, z.grid, z.slots);
 }
 
 }  // namespace

@@ -146,22 +146,28 @@ __global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, uint32_t*
   }
 }
 
-// One CTA per (request, key head): the key of the top-th best page by four
-// passes over 8 bits of the keys, then the pages above it and the lowest pages
-// at it, in ascending order.
+// One CTA per (request, key head): the key of the last page to take by passes
+// over 8 bits of the keys, then the pages above it and the lowest pages at it, in
+// ascending order. The bits are those of the keys' own range (scores of one row
+// share their upper bits: counting those would put all keys into one bin, one
+// after the other), and the passes end once a bin is taken whole, for a thousand
+// pages usually after two.
 __global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a,
                                                               const uint32_t* __restrict__ row_keys) {
+  constexpr int kTopWarps = kTopThreads / 32;
   __shared__ int hist[256];
-  __shared__ int sh_bin, sh_left;
-  __shared__ int wsum[2][kTopThreads / 32];
+  __shared__ int sh_bin, sh_left, sh_count;
+  __shared__ uint32_t wred[2][kTopWarps];
+  __shared__ int wsum[2][2][kTopWarps];
   __shared__ uint32_t keys[kTopKeys];
   pdl_wait();
   const int row = blockIdx.x;
   const int b = row / a.pool.Hk;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int pl = a.pool.page_len;
-  if (a.lens[b] > a.max_pages * pl && threadIdx.x == 0) set_status(a.status, SAGA_STATUS_PAGE_RANGE);
-  const int len = min(max(a.lens[b], 0), a.max_pages * pl);
+  const int given = a.lens[b];
+  if (given > a.max_pages * pl && threadIdx.x == 0) set_status(a.status, SAGA_STATUS_PAGE_RANGE);
+  const int len = min(max(given, 0), a.max_pages * pl);
   const int pages = (len + pl - 1) / pl;
   int32_t* out = a.blocks + (int64_t)row * a.top;
   if (threadIdx.x == 0) a.counts[row] = min(pages, a.top);
@@ -170,19 +176,37 @@ __global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a,
     return;
   }
   const uint32_t* s = row_keys + (int64_t)row * a.max_pages;
-  auto make_key = [&](int j) -> uint32_t {
-    return (j < a.keep_first || j >= pages - a.keep_last) ? 0xffffffffu : s[j];
-  };
-  for (int j = threadIdx.x; j < min(pages, kTopKeys); j += kTopThreads) keys[j] = make_key(j);
-  auto key_of = [&](int j) -> uint32_t { return j < kTopKeys ? keys[j] : make_key(j); };
-  uint32_t prefix = 0;
-  int left = a.top;  // pages still to take among those that match the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kTopThreads) hist[i] = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < pages; j += kTopThreads) {
-      const uint32_t k = key_of(j);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
+  const int j0 = a.keep_first, j1 = pages - a.keep_last;  // the scored pages: [j0, j1)
+  uint32_t least = 0xffffffffu, most = 0u;
+  for (int j = j0 + threadIdx.x; j < j1; j += kTopThreads) {
+    const uint32_t k = s[j];
+    if (j < kTopKeys) keys[j] = k;
+    least = min(least, k);
+    most = max(most, k);
+  }
+  auto key_of = [&](int j) -> uint32_t { return j < kTopKeys ? keys[j] : s[j]; };
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) {
+    wred[0][warp] = least;
+    wred[1][warp] = most;
+  }
+  for (int i = threadIdx.x; i < 256; i += kTopThreads) hist[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kTopWarps; ++w) {
+    least = min(least, wred[0][w]);
+    most = max(most, wred[1][w]);
+  }
+  int left = a.top - (a.keep_first + a.keep_last);  // scored pages to take among those that match `pre`
+  int shift = j0 < j1 && most > least ? 32 - __clz(most - least) : 0;
+  uint32_t pre = 0;  // key - least, shifted, of the bin that holds the last one
+  while (shift > 0 && left > 0) {
+    const int width = min(8, shift), up = shift;
+    shift -= width;
+    for (int j = j0 + threadIdx.x; j < j1; j += kTopThreads) {
+      const uint32_t d = key_of(j) - least;
+      if ((uint32_t)((uint64_t)d >> up) == pre) atomicAdd(&hist[(d >> shift) & ((1u << width) - 1u)], 1);
     }
     __syncthreads();
     if (warp == 0) {  // the bin that holds the left-th greatest: lane l has bins 255 - 8l .. 248 - 8l
@@ -195,40 +219,44 @@ __global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a,
         if (above < left && left <= above + c[i]) {
           sh_bin = 255 - 8 * lane - i;
           sh_left = left - above;
+          sh_count = c[i];
         }
         above += c[i];
+        hist[255 - 8 * lane - i] = 0;  // for the next pass
       }
     }
     __syncthreads();
-    prefix |= (uint32_t)sh_bin << shift;
+    pre = (pre << width) | (uint32_t)sh_bin;
     left = sh_left;
+    if (sh_count == left) break;  // the bin is taken whole
   }
   int done_gt = 0, done_eq = 0;  // pages above the key and at it so far
-  for (int base = 0; base < pages; base += kTopThreads) {
+  int turn = 0;
+  for (int base = 0; base < pages; base += kTopThreads, turn ^= 1) {
     const int j = base + threadIdx.x;
-    const uint32_t k = j < pages ? key_of(j) : 0u;
-    const bool gt = k > prefix, eq = j < pages && k == prefix;
+    const bool scored = j >= j0 && j < j1;
+    const uint32_t d = scored ? (key_of(j) - least) >> shift : 0u;
+    const bool gt = j < pages && (!scored || d > pre), eq = scored && d == pre;
     const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) {
-      wsum[0][warp] = __popc(bg);
-      wsum[1][warp] = __popc(be);
+      wsum[turn][0][warp] = __popc(bg);
+      wsum[turn][1][warp] = __popc(be);
     }
-    __syncthreads();
+    __syncthreads();  // the other half of wsum is written next: one barrier per round
     int g = done_gt, e = done_eq;
 #pragma unroll
-    for (int w = 0; w < kTopThreads / 32; ++w) {
+    for (int w = 0; w < kTopWarps; ++w) {
       if (w < warp) {
-        g += wsum[0][w];
-        e += wsum[1][w];
+        g += wsum[turn][0][w];
+        e += wsum[turn][1][w];
       }
-      done_gt += wsum[0][w];
-      done_eq += wsum[1][w];
+      done_gt += wsum[turn][0][w];
+      done_eq += wsum[turn][1][w];
     }
     const unsigned below = (1u << lane) - 1u;
     g += __popc(bg & below);
     e += __popc(be & below);
     if (gt || (eq && e < left)) out[g + min(e, left)] = j;
-    __syncthreads();
   }
 }
 
