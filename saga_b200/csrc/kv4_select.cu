@@ -39,14 +39,15 @@ __device__ __forceinline__ float warp_sums4(float (&v)[4]) {
   return s;
 }
 
-constexpr int kScorePages = 4;  // pages per warp, at most
+constexpr int kScoreBatch = 2;  // pages whose bounds a warp loads together
+constexpr int kScorePages = 8;  // pages per warp, at most (a multiple of the batch)
 
 // A warp scores `per_warp` consecutive pages for the heads of one key head, 4 NC
 // of them at a time in registers: lane l has channels l, l + 32 (l + 64, l + 96),
 // so the first levels of the tree are its own and the last five go across the
 // warp. Scores are written as keys.
 template <typename T, int D, int NC>
-__global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, uint32_t* __restrict__ keys, int per_warp) {
+__global__ void __launch_bounds__(256, 3) kv4_score_kernel(SagaKv4Args a, uint32_t* __restrict__ keys, int per_warp) {
   constexpr int N = D / 32, NV = 4 * NC;
   __shared__ float qs[NV][D];
   pdl_wait();
@@ -70,26 +71,8 @@ __global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, uint32_t*
       mine = 0;
     }
   }
-  // the bounds of all its pages are on their way while the queries are staged
-  __nv_bfloat16 lo[kScorePages][N], hi[kScorePages][N];
-#pragma unroll
-  for (int x = 0; x < kScorePages; ++x) {
-    const int page = __shfl_sync(0xffffffffu, mine, x);
-    if (x < n) {
-      const int64_t at = ((int64_t)page * a.pool.Hk + kh) * D + lane;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        lo[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_lo)[at + 32 * i];
-        hi[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_hi)[at + 32 * i];
-      }
-    }
-  }
   const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)kh * G * a.q_sh;
-  uint32_t best[kScorePages];
-#pragma unroll
-  for (int x = 0; x < kScorePages; ++x) best[x] = 0u;
-  bool nan[kScorePages] = {};
-  for (int g0 = 0; g0 < G; g0 += NV) {
+  auto stage = [&](int g0) {
     // one coalesced load of the queries per CTA: a warp's own 2-byte loads of all heads took longer than its pages
     __syncthreads();
     for (int x = threadIdx.x; x < NV * D; x += 256) {
@@ -97,52 +80,75 @@ __global__ void __launch_bounds__(256) kv4_score_kernel(SagaKv4Args a, uint32_t*
       qs[g][d] = g0 + g < G ? Num<T>::to_f(q[(int64_t)(g0 + g) * a.q_sh + d]) : 0.f;
     }
     __syncthreads();
-    f32x2 qv[NV][N / 2];
+  };
+  for (int p0 = 0; p0 < per_warp; p0 += kScoreBatch) {  // the same trips for all warps: the staging has barriers
+    // the bounds of a batch of pages are on their way together, at first while the queries are staged
+    __nv_bfloat16 lo[kScoreBatch][N], hi[kScoreBatch][N];
 #pragma unroll
-    for (int g = 0; g < NV; ++g)
+    for (int x = 0; x < kScoreBatch; ++x) {
+      const int page = __shfl_sync(0xffffffffu, mine, (p0 + x) & 31);
+      if (p0 + x < n) {
+        const int64_t at = ((int64_t)page * a.pool.Hk + kh) * D + lane;
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) qv[g][i] = pack2(qs[g][lane + 64 * i], qs[g][lane + 64 * i + 32]);
-#pragma unroll
-    for (int x = 0; x < kScorePages; ++x) {
-      if (x >= n) break;
-      f32x2 l[N / 2], h[N / 2];
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        l[i] = pack2(__bfloat162float(lo[x][2 * i]), __bfloat162float(lo[x][2 * i + 1]));
-        h[i] = pack2(__bfloat162float(hi[x][2 * i]), __bfloat162float(hi[x][2 * i + 1]));
-      }
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float s[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          // lo <= hi, so the greater of the two products is the one that the sign of q picks
-          f32x2 y[N / 2];
-#pragma unroll
-          for (int i = 0; i < N / 2; ++i) {
-            float h0, h1, l0, l1;
-            unpack2(mul2(qv[4 * c + g][i], h[i]), h0, h1);
-            unpack2(mul2(qv[4 * c + g][i], l[i]), l0, l1);
-            y[i] = pack2(fmaxf(h0, l0), fmaxf(h1, l1));
-          }
-          if constexpr (N == 4) y[0] = add2(y[0], y[N / 2 - 1]);  // channels d and d + 64
-          float y0, y1;
-          unpack2(y[0], y0, y1);
-          s[g] = __fadd_rn(y0, y1);  // d and d + 32
+        for (int i = 0; i < N; ++i) {
+          lo[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_lo)[at + 32 * i];
+          hi[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_hi)[at + 32 * i];
         }
-        const float t = warp_sums4(s);
-        const bool real = g0 + 4 * c + lane / 8 < G;
-        nan[x] |= real && t != t;
-        best[x] = max(best[x], real ? score_key(t) : 0u);
       }
     }
-  }
+    uint32_t best[kScoreBatch];
+    bool nan[kScoreBatch];
 #pragma unroll
-  for (int x = 0; x < kScorePages; ++x) {
-    if (x >= n) break;
-    uint32_t key = __reduce_max_sync(0xffffffffu, best[x]);
-    if (__any_sync(0xffffffffu, nan[x])) key = kNanKey;
-    if (lane == 0) keys[(int64_t)row * a.max_pages + j0 + x] = key;
+    for (int x = 0; x < kScoreBatch; ++x) {
+      best[x] = 0u;
+      nan[x] = false;
+    }
+    for (int g0 = 0; g0 < G; g0 += NV) {
+      if (p0 == 0 || G > NV) stage(g0);
+      // four heads at a time from shared memory, for all pages of the batch: with all heads in registers
+      // one CTA filled an SM, and its warps waited for one another's loads
+#pragma unroll 1
+      for (int c = 0; c < NC; ++c) {
+        f32x2 qv[4][N / 2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i)
+            qv[g][i] = pack2(qs[4 * c + g][lane + 64 * i], qs[4 * c + g][lane + 64 * i + 32]);
+        const bool real = g0 + 4 * c + lane / 8 < G;
+#pragma unroll
+        for (int x = 0; x < kScoreBatch; ++x) {
+          if (p0 + x >= n) break;
+          float s[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            // lo <= hi, so the greater of the two products is the one that the sign of q picks
+            f32x2 y[N / 2];
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+              float h0, h1, l0, l1;
+              unpack2(mul2(qv[g][i], pack2(__bfloat162float(hi[x][2 * i]), __bfloat162float(hi[x][2 * i + 1]))), h0, h1);
+              unpack2(mul2(qv[g][i], pack2(__bfloat162float(lo[x][2 * i]), __bfloat162float(lo[x][2 * i + 1]))), l0, l1);
+              y[i] = pack2(fmaxf(h0, l0), fmaxf(h1, l1));
+            }
+            if constexpr (N == 4) y[0] = add2(y[0], y[N / 2 - 1]);  // channels d and d + 64
+            float y0, y1;
+            unpack2(y[0], y0, y1);
+            s[g] = __fadd_rn(y0, y1);  // d and d + 32
+          }
+          const float t = warp_sums4(s);
+          nan[x] |= real && t != t;
+          best[x] = max(best[x], real ? score_key(t) : 0u);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kScoreBatch; ++x) {
+      if (p0 + x >= n) break;
+      uint32_t key = __reduce_max_sync(0xffffffffu, best[x]);
+      if (__any_sync(0xffffffffu, nan[x])) key = kNanKey;
+      if (lane == 0) keys[(int64_t)row * a.max_pages + j0 + p0 + x] = key;
+    }
   }
 }
 
@@ -272,7 +278,7 @@ int launch_kv4_select(const SagaKv4Args& a, cudaStream_t st) {
   const int G = a.Hq / a.pool.Hk;
   if (rows > 65535) return abi_fail(SAGA_ERR_UNSUPPORTED, "more than 65535 (request, key head) rows");
   if (a.max_pages > a.top) {
-    // one page per warp where the SMs hold that many warps (two CTAs of eight each), else up to four
+    // one page per warp where the SMs hold that many warps, else up to eight
     const int64_t warps = (int64_t)rows * a.max_pages;
     const int per_warp = (int)std::min<int64_t>(kScorePages, (warps + 16 * 148 - 1) / (16 * 148));
     const dim3 grid((a.max_pages + 8 * per_warp - 1) / (8 * per_warp), rows);
