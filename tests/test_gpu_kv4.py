@@ -839,3 +839,17 @@ def test_compiled_step_matches_eager():
         results.append([t.clone() for t in (*outs, c.table, c.device_lens, state, c.pool.k, c.pool.v)])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("top", [0, 6])
+def test_serving_example(top):
+    """The example's loop: lengths, pages and attention are right after admissions, steps and a finished
+    request. With values of unit range in 15 steps, a rounding error of at most half a step on keys and values
+    stays well below the signal; over all pages the outputs are close to the 16-bit ones."""
+    from saga_b200.serve_kv4 import serve
+    r = serve(requests=5, prompt=700, steps=40, top=top, page_len=32)
+    assert r["lens"] == r["expected_lens"] and r["status"] == 0
+    assert r["pages_held"] + r["pages_free"] == r["pages"]
+    assert r["cache_bytes"] < 0.35 * r["cache_bytes_16bit"]  # 9/32 of it, and pages partly filled
+    if not top:
+        assert r["cosine_to_16bit"] > 0.97
