@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -40,19 +41,23 @@ struct Pool {
   std::map<std::vector<int64_t>, size_t> sizes;  // workspace bytes per op and shapes
 };
 
-// Workspaces per (device, stream). The kernels do not care what one holds.
-// Smaller ones are kept, since a CUDA graph may refer to them.
-std::map<std::pair<int, cudaStream_t>, std::vector<at::Tensor>>& scratches() {
-  static auto* m = new std::map<std::pair<int, cudaStream_t>, std::vector<at::Tensor>>();  // outlives CUDA's teardown
+// A workspace for one call on the current stream: one is kept per (device,
+// stream), since calls in a stream do not overlap. A call under capture gets one
+// of its own from the graph's memory: graphs captured on one stream may be
+// replayed on several. The kernels do not care what a workspace holds.
+std::map<std::pair<int, cudaStream_t>, at::Tensor>& scratches() {
+  static auto* m = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();  // outlives CUDA's teardown
   return *m;
 }
-void* scratch(int index, cudaStream_t stream, size_t nbytes) {
-  auto& have = scratches()[{index, stream}];
-  if (have.empty() || (size_t)have.back().numel() < nbytes) {
-    const size_t grown = std::max(nbytes, have.empty() ? (size_t)1 << 20 : 2 * (size_t)have.back().numel());
-    have.push_back(at::empty({(int64_t)grown}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, index)));
-  }
-  return have.back().data_ptr();
+at::Tensor scratch(int index, cudaStream_t stream, size_t nbytes) {
+  auto take = [&](size_t n) {
+    return at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, index));
+  };
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return take(nbytes);
+  at::Tensor& have = scratches()[{index, stream}];
+  if (!have.defined()) have = take(std::max(nbytes, (size_t)1 << 20));
+  else if ((size_t)have.numel() < nbytes) have = take(std::max(nbytes, 2 * (size_t)have.numel()));
+  return have;
 }
 
 int dtype_code(at::ScalarType t) {
@@ -142,14 +147,14 @@ PyObject* py_pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
                        [](PyObject* c) { delete reinterpret_cast<Pool*>(PyCapsule_GetPointer(c, "saga_kv4_pool")); });
 }
 
-// scratch(device index, stream, bytes): the address of a workspace
+// scratch(device index, stream, bytes): a workspace, to be held until the call has been made
 PyObject* py_scratch(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 3) return PyErr_Format(PyExc_TypeError, "scratch takes three arguments");
   const int index = (int)PyLong_AsLong(a[0]);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(PyLong_AsVoidPtr(a[1]));
   const size_t bytes = PyLong_AsSize_t(a[2]);
   if (PyErr_Occurred()) return nullptr;
-  return guarded([&] { return PyLong_FromVoidPtr(scratch(index, st, bytes)); });
+  return guarded([&] { return THPVariable_Wrap(scratch(index, st, bytes)); });
 }
 
 // write(pool, k, v, slots) -> True
@@ -227,7 +232,8 @@ int run(Pool* p, SagaKv4Args* c, int op) {
   if (!bytes) bytes = f_workspace(c, op);
   if (!bytes) return -1;
   cudaStream_t st = stream_of(p->index);
-  c->workspace = scratch(p->index, st, bytes);
+  const at::Tensor ws = scratch(p->index, st, bytes);
+  c->workspace = ws.data_ptr();
   c->workspace_bytes = bytes;
   return op == SAGA_KV4_DECODE ? f_decode(c, st) : f_select(c, st);
 }
@@ -350,7 +356,8 @@ PyObject* py_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c.status = reinterpret_cast<int32_t*>(PyLong_AsVoidPtr(a[9]));
     cudaStream_t st = stream_of(index);
     c.workspace_bytes = 16 * (size_t)B;
-    c.workspace = scratch(index, st, c.workspace_bytes);
+    const at::Tensor ws = scratch(index, st, c.workspace_bytes);
+    c.workspace = ws.data_ptr();
     if (f_tables(&c, st)) SLOW_PATH;
     PyObject* r = PyTuple_New(5);
     if (!r) return nullptr;

@@ -277,7 +277,8 @@ def _kv4_run(fn, name: str, a: L.SagaKv4Args, op: int, pool: Kv4Pool) -> None:
         if nbytes == 0:
             raise L.SagaError(L.SAGA_ERR_INVALID, "saga_kv4_workspace_bytes")
         stream = _raw_stream(index)
-        a.workspace = _fast.scratch(index, stream, nbytes)
+        workspace = _fast.scratch(index, stream, nbytes)
+        a.workspace = workspace.data_ptr()
         a.workspace_bytes = nbytes
         rc = fn(ref, stream)
     if rc:
@@ -430,7 +431,8 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     nbytes = max(16 * B, 16)
     with _on_device(index):
         stream = _raw_stream(index)
-        a.workspace = _fast.scratch(index, stream, nbytes)
+        workspace = _fast.scratch(index, stream, nbytes)
+        a.workspace = workspace.data_ptr()
         a.workspace_bytes = nbytes
         rc = L.lib.saga_page_tables(ctypes.byref(a), stream)
     if rc:

@@ -719,6 +719,29 @@ def test_calls_on_two_streams_do_not_share_a_workspace():
         assert all(torch.equal(a, b) for a, b in zip(outs, ref))
 
 
+def test_graphs_captured_on_one_stream_do_not_share_a_workspace():
+    from saga_b200 import kv4
+    caches = [Cache([20000 + i, 300], 1, 2, 128, 128, seed=70 + i) for i in range(2)]
+    qs = [torch.randn((2, 12, 1, 128), generator=gen(80 + i), device=DEV).to(torch.bfloat16) for i in range(2)]
+    ref = [kv4.kv4_decode(q, c.pool, c.table, c.device_lens) for q, c in zip(qs, caches)]
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, q, c in zip(graphs, qs, caches):
+        with torch.cuda.graph(graph):
+            outs.append(kv4.kv4_decode(q, c.pool, c.table, c.device_lens))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, r in zip(outs, ref):
+            assert torch.equal(o, r)
+
+
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
