@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kTopThreads) kv4_top_kernel(SagaKv4Args a,
   for (int base = 0; base < pages; base += kTopThreads, turn ^= 1) {
     const int j = base + threadIdx.x;
     const bool scored = j >= j0 && j < j1;
-    const uint32_t d = scored ? (key_of(j) - least) >> shift : 0u;
+    const uint32_t d = scored ? (uint32_t)((uint64_t)(key_of(j) - least) >> shift) : 0u;  // shift: up to 32
     const bool gt = j < pages && (!scored || d > pre), eq = scored && d == pre;
     const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) {

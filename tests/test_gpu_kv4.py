@@ -503,6 +503,23 @@ def test_pages_of_nan_keys_are_selected_last():
     assert blocks[0, 0].tolist() == [0, 1, 2, 3, 4, 5, 7, 8, 9]
 
 
+def test_select_nothing_between_the_kept_pages():
+    """No scored page is taken; the scores have both signs, so their keys' range has 32 bits."""
+    from saga_b200 import kv4
+    d, pl, n = 64, 32, 40
+    pool = kv4.Kv4Pool(n, pl, 1, 1, d, device=DEV, bounds=True)
+    table = torch.arange(n, dtype=torch.int32, device=DEV)[None]
+    lens = torch.tensor([n * pl], dtype=torch.int32, device=DEV)
+    x = torch.linspace(-2e30, 2e30, n, device=DEV).to(torch.bfloat16)
+    pool.k_lo.copy_(x[:, None, None].expand_as(pool.k_lo))
+    pool.k_hi.copy_(pool.k_lo)
+    q = torch.ones((1, 2, 1, d), device=DEV, dtype=torch.bfloat16)
+    for first, last in ((2, 1), (0, 1), (1, 3)):
+        blocks, counts = kv4.kv4_select(q, pool, table, lens, first + last, keep_first=first, keep_last=last)
+        assert blocks[0, 0].tolist() == list(range(first)) + list(range(n - last, n))
+        assert int(counts[0, 0]) == first + last
+
+
 def test_select_more_pages_than_fit_shared_memory():
     from saga_b200 import kv4
     d, pl, n, top = 64, 32, 9000, 50
