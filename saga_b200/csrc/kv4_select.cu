@@ -49,7 +49,7 @@ constexpr int kScorePages = 8;  // pages per warp, at most (a multiple of the ba
 template <typename T, int D, int NC>
 __global__ void __launch_bounds__(256, 3) kv4_score_kernel(SagaKv4Args a, uint32_t* __restrict__ keys, int per_warp) {
   constexpr int N = D / 32, NV = 4 * NC;
-  __shared__ float qs[NV][D];
+  __shared__ __align__(16) float qs[NV][32][N];  // a lane's channels are one load
   pdl_wait();
   const int G = a.Hq / a.pool.Hk;
   const int row = blockIdx.y;
@@ -77,13 +77,14 @@ __global__ void __launch_bounds__(256, 3) kv4_score_kernel(SagaKv4Args a, uint32
     __syncthreads();
     for (int x = threadIdx.x; x < NV * D; x += 256) {
       const int g = x / D, d = x % D;
-      qs[g][d] = g0 + g < G ? Num<T>::to_f(q[(int64_t)(g0 + g) * a.q_sh + d]) : 0.f;
+      qs[g][d % 32][d / 32] = g0 + g < G ? Num<T>::to_f(q[(int64_t)(g0 + g) * a.q_sh + d]) : 0.f;
     }
     __syncthreads();
   };
-  for (int p0 = 0; p0 < per_warp; p0 += kScoreBatch) {  // the same trips for all warps: the staging has barriers
-    // the bounds of a batch of pages are on their way together, at first while the queries are staged
-    __nv_bfloat16 lo[kScoreBatch][N], hi[kScoreBatch][N];
+  // the bounds of a batch of pages are on their way together, while the queries are staged or the batch
+  // before it is scored
+  __nv_bfloat16 lo[kScoreBatch][N], hi[kScoreBatch][N], lo_next[kScoreBatch][N], hi_next[kScoreBatch][N];
+  auto fetch = [&](int p0) {
 #pragma unroll
     for (int x = 0; x < kScoreBatch; ++x) {
       const int page = __shfl_sync(0xffffffffu, mine, (p0 + x) & 31);
@@ -91,20 +92,32 @@ __global__ void __launch_bounds__(256, 3) kv4_score_kernel(SagaKv4Args a, uint32
         const int64_t at = ((int64_t)page * a.pool.Hk + kh) * D + lane;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          lo[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_lo)[at + 32 * i];
-          hi[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_hi)[at + 32 * i];
+          lo_next[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_lo)[at + 32 * i];
+          hi_next[x][i] = reinterpret_cast<const __nv_bfloat16*>(a.pool.k_hi)[at + 32 * i];
         }
       }
     }
-    uint32_t best[kScoreBatch];
+  };
+  fetch(0);
+  for (int p0 = 0; p0 < per_warp; p0 += kScoreBatch) {  // the same trips for all warps: the staging has barriers
+    if (p0 == 0) stage(0);
+#pragma unroll
+    for (int x = 0; x < kScoreBatch; ++x)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        lo[x][i] = lo_next[x][i];
+        hi[x][i] = hi_next[x][i];
+      }
+    fetch(p0 + kScoreBatch);
+    float best[kScoreBatch];
     bool nan[kScoreBatch];
 #pragma unroll
     for (int x = 0; x < kScoreBatch; ++x) {
-      best[x] = 0u;
+      best[x] = -INFINITY;
       nan[x] = false;
     }
     for (int g0 = 0; g0 < G; g0 += NV) {
-      if (p0 == 0 || G > NV) stage(g0);
+      if (G > NV) stage(g0);
       // four heads at a time from shared memory, for all pages of the batch: with all heads in registers
       // one CTA filled an SM, and its warps waited for one another's loads
 #pragma unroll 1
@@ -114,7 +127,7 @@ __global__ void __launch_bounds__(256, 3) kv4_score_kernel(SagaKv4Args a, uint32
         for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int i = 0; i < N / 2; ++i)
-            qv[g][i] = pack2(qs[4 * c + g][lane + 64 * i], qs[4 * c + g][lane + 64 * i + 32]);
+            qv[g][i] = reinterpret_cast<const f32x2*>(qs[4 * c + g][lane])[i];
         const bool real = g0 + 4 * c + lane / 8 < G;
 #pragma unroll
         for (int x = 0; x < kScoreBatch; ++x) {
@@ -138,14 +151,14 @@ __global__ void __launch_bounds__(256, 3) kv4_score_kernel(SagaKv4Args a, uint32
           }
           const float t = warp_sums4(s);
           nan[x] |= real && t != t;
-          best[x] = max(best[x], real ? score_key(t) : 0u);
+          if (real) best[x] = fmaxf(best[x], t);
         }
       }
     }
 #pragma unroll
     for (int x = 0; x < kScoreBatch; ++x) {
       if (p0 + x >= n) break;
-      uint32_t key = __reduce_max_sync(0xffffffffu, best[x]);
+      uint32_t key = __reduce_max_sync(0xffffffffu, score_key(best[x]));
       if (__any_sync(0xffffffffu, nan[x])) key = kNanKey;
       if (lane == 0) keys[(int64_t)row * a.max_pages + j0 + p0 + x] = key;
     }
