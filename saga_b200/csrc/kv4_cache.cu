@@ -14,8 +14,11 @@ namespace {
 // per group and leave as two words of codes per lane, 32 consecutive bytes (one
 // sector) per group. What is done once per group (the address, the scale) costs
 // as much as ten values, so fewer lanes with more values each are cheaper: eight
-// lanes of eight values took 98 us where these take 56 us (131,072 tokens, five
-// heads of 128, bf16: 215 MB).
+// lanes of eight values took 98 us where these take 51 us (131,072 tokens, five
+// heads of 128, bf16: 215 MB, 4.2 TB/s). The write is bound by its instructions
+// (the schedulers issue in 83 % of the cycles), the read, 40 us, by its stores
+// (5.4 TB/s). The rows go past the caches (__ldcs, __stcs): a prompt's rows are
+// larger than L2, and the read took 43 us without.
 constexpr int kLanes = 4;
 constexpr int kCtaThreads = 256;
 constexpr int kCtaGroups = kCtaThreads / kLanes;
@@ -33,7 +36,7 @@ __device__ __forceinline__ void load16(const T* p, Raw<T>& r) {
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        r.w[h * sizeof(T) / 2 + i] = reinterpret_cast<const uint4*>(p + 32 * h)[i];
+        r.w[h * sizeof(T) / 2 + i] = __ldcs(reinterpret_cast<const uint4*>(p + 32 * h) + i);
     } else {
       T* t = reinterpret_cast<T*>(&r) + 8 * h;
 #pragma unroll
@@ -48,7 +51,7 @@ __device__ __forceinline__ void store16(T* p, const Raw<T>& r) {
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        reinterpret_cast<uint4*>(p + 32 * h)[i] = r.w[h * sizeof(T) / 2 + i];
+        __stcs(reinterpret_cast<uint4*>(p + 32 * h) + i, r.w[h * sizeof(T) / 2 + i]);
     } else {
       const T* t = reinterpret_cast<const T*>(&r) + 8 * h;
 #pragma unroll
@@ -207,6 +210,20 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_write_kernel(const T* __restr
   }
 }
 
+// The eight codes of a word as pairs of binary32 values: y[j] has codes j and j + 4.
+// Put into the low bits of the fp16 number 1024, a code (or 16 times a code) is
+// exact; in that form two take one logical and one fp16 instruction.
+__device__ __forceinline__ void codes8(uint32_t w, f32x2 (&y)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t u = (j < 2 ? w : w >> 8) & (j & 1 ? 0x00f000f0u : 0x000f000fu) | 0x64006400u;
+    const __half2 one = __floats2half2_rn(j & 1 ? 0.0625f : 1.f, j & 1 ? 0.0625f : 1.f);
+    const __half2 off = __floats2half2_rn(j & 1 ? -64.f : -1024.f, j & 1 ? -64.f : -1024.f);
+    const float2 c = __half22float2(__hfma2(*reinterpret_cast<const __half2*>(&u), one, off));
+    y[j] = pack2(c.x, c.y);
+  }
+}
+
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k, T* __restrict__ v, Rows kr, Rows vr,
                                                                Deal deal, const int64_t* __restrict__ slots,
@@ -233,16 +250,19 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
       const float s = kv4_scale(m[i]), z = kv4_zero(m[i]);
       Raw<T> r;
       T* x = reinterpret_cast<T*>(&r);
-      const f32x2 s2 = pack2(s, s), z2 = pack2(z, z), magic = pack2(-kMagic, -kMagic);
+      const f32x2 s2 = pack2(s, s), z2 = pack2(z, z);
       // s * code has at most 12 significant bits, so the sum is rounded once
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const uint32_t c = w[i][j / 8] >> (4 * (j % 8));
-        const f32x2 y = pack2(__uint_as_float((c & 15u) | 0x4b000000u), __uint_as_float(((c >> 4) & 15u) | 0x4b000000u));
-        float y0, y1;
-        unpack2(fma2(s2, add2(y, magic), z2), y0, y1);
-        x[j] = Num<T>::from_f(y0);
-        x[j + 1] = Num<T>::from_f(y1);
+      for (int h = 0; h < 2; ++h) {
+        f32x2 y[4];
+        codes8(w[i][h], y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y0, y1;
+          unpack2(fma2(s2, y[j], z2), y0, y1);
+          x[8 * h + j] = Num<T>::from_f(y0);
+          x[8 * h + j + 4] = Num<T>::from_f(y1);
+        }
       }
       store16<T, VEC>((at[i].is_v ? v : k) + at[i].src, r);
     }
@@ -251,26 +271,27 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
 
 // Bounds of the pages whose last slot is among the slots: a CTA looks at
 // `strip` tokens and takes the bounds of the pages that they complete. Threads
-// split a page into D/8 words of a row by 16 (32) rows.
+// split a page into D/8 words of a row by 16 (32) rows. 1024 pages of 128 rows of
+// 128 take 10 us after the write that completes them (one page at a time and its
+// loads' latency: the schedulers issue in 38 % of the cycles); four rows of a
+// thread on their way together, since eight need 80 registers and leave fewer
+// CTAs per SM (13 us).
 constexpr int kBoundThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kBoundThreads) kv4_bounds_kernel(SagaKv4Pool p, int64_t T_, int strip,
                                                          const int64_t* __restrict__ slots) {
   constexpr int W = D / 8, ROWS = kBoundThreads / W;
-  __shared__ float red[2][ROWS][D];
-  pdl_wait();
-  __shared__ int64_t done[32];
+  __shared__ __align__(16) float red[2][ROWS][D];
+  __shared__ int64_t done[kBoundThreads];
   __shared__ int n_done;
+  if (threadIdx.x == 0) n_done = 0;
+  pdl_wait();
+  __syncthreads();
   const int w = threadIdx.x % W, rr = threadIdx.x / W;
-  if (threadIdx.x < 32) {  // strip <= 32
-    const int64_t t = (int64_t)blockIdx.x * strip + threadIdx.x;
-    const int64_t slot = (int)threadIdx.x < strip && t < T_ ? slots[t] : -1;
-    const bool last = slot >= 0 && slot < (int64_t)p.num_pages * p.page_len &&
-                      (slot & (p.page_len - 1)) == p.page_len - 1;
-    const unsigned all = __ballot_sync(0xffffffffu, last);
-    if (last) done[__popc(all & ((1u << threadIdx.x) - 1u))] = slot / p.page_len;
-    if (threadIdx.x == 0) n_done = __popc(all);
-  }
+  const int64_t t = (int64_t)blockIdx.x * strip + threadIdx.x;
+  const int64_t slot = (int)threadIdx.x < strip && t < T_ ? slots[t] : -1;
+  if (slot >= 0 && slot < (int64_t)p.num_pages * p.page_len && (slot & (p.page_len - 1)) == p.page_len - 1)
+    done[atomicAdd(&n_done, 1)] = slot / p.page_len;  // in any order: each page is by itself
   __syncthreads();
   const int n = n_done;
   for (int x = 0; x < n; ++x) {
@@ -282,7 +303,7 @@ __global__ void __launch_bounds__(kBoundThreads) kv4_bounds_kernel(SagaKv4Pool p
         lo[i] = INFINITY;
         hi[i] = -INFINITY;
       }
-#pragma unroll 8
+#pragma unroll 4
       for (int off = rr; off < p.page_len; off += ROWS) {
         const uint8_t* tile =
             reinterpret_cast<const uint8_t*>(p.k) + kv4_tile_at<D>(page, h, p.Hk, off, p.page_len);
@@ -291,17 +312,23 @@ __global__ void __launch_bounds__(kBoundThreads) kv4_bounds_kernel(SagaKv4Pool p
             *reinterpret_cast<const uint32_t*>(tile + kv4_chunk_off<D>(row, w >> 2) + (w & 3) * 4);
         const uint32_t m = *reinterpret_cast<const uint32_t*>(tile + kv4_meta_off<D>(row, w >> 3));
         const float s = kv4_scale(m), z = kv4_zero(m);
+        const f32x2 s2 = pack2(s, s), z2 = pack2(z, z);
+        f32x2 y[4];
+        codes8(c, y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // NaN rows are left out (fminf and fmaxf return the other operand)
-          const float x = __fmaf_rn(s, __uint_as_float(((c >> (4 * i)) & 15u) | 0x4b000000u) - kMagic, z);
-          lo[i] = fminf(lo[i], x);
-          hi[i] = fmaxf(hi[i], x);
+        for (int j = 0; j < 4; ++j) {  // NaN rows are left out (fminf and fmaxf return the other operand)
+          float x0, x1;
+          unpack2(fma2(s2, y[j], z2), x0, x1);
+          lo[j] = fminf(lo[j], x0);
+          hi[j] = fmaxf(hi[j], x0);
+          lo[j + 4] = fminf(lo[j + 4], x1);
+          hi[j + 4] = fmaxf(hi[j + 4], x1);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        red[0][rr][w * 8 + i] = lo[i];
-        red[1][rr][w * 8 + i] = hi[i];
+      for (int i = 0; i < 8; i += 4) {  // the word's fourths of all words together: no bank conflicts
+        *reinterpret_cast<float4*>(&red[0][rr][i * W + 4 * w]) = make_float4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
+        *reinterpret_cast<float4*>(&red[1][rr][i * W + 4 * w]) = make_float4(hi[i], hi[i + 1], hi[i + 2], hi[i + 3]);
       }
       __syncthreads();
       if (threadIdx.x < D) {
@@ -312,7 +339,8 @@ __global__ void __launch_bounds__(kBoundThreads) kv4_bounds_kernel(SagaKv4Pool p
           b = fmaxf(b, red[1][i][threadIdx.x]);
         }
         if (a > b) a = b = __int_as_float(0x7fffffff);  // no key stands for a number here
-        const int64_t at = (page * p.Hk + h) * D + threadIdx.x;
+        const int d = (int)threadIdx.x % (4 * W) / 4 * 8 + (int)threadIdx.x / (4 * W) * 4 + (int)threadIdx.x % 4;
+        const int64_t at = (page * p.Hk + h) * D + d;
         reinterpret_cast<__nv_bfloat16*>(p.k_lo)[at] = bf16_down(a);
         reinterpret_cast<__nv_bfloat16*>(p.k_hi)[at] = bf16_up(b);
       }
@@ -380,8 +408,8 @@ int launch_kv4_write(const SagaKv4Pool& p, int dt, int64_t T, const void* k, int
                     reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v), kr, vr, deal, slots, status);
   });
   if (rc || !p.k_lo) return rc;
-  // one token per CTA where every token may complete a page; runs of prompt tokens complete one in 32 at most
-  const int strip = T <= 4096 ? 1 : 32;
+  // one token per CTA where every token may complete a page; a run of prompt tokens completes one in page_len
+  const int strip = T <= 4096 ? 1 : std::min(p.page_len, kBoundThreads);
   const unsigned nb = (unsigned)((T + strip - 1) / strip);
   return kv4_launch("kv4_bounds_kernel", p.D == 128 ? kv4_bounds_kernel<128> : kv4_bounds_kernel<64>, dim3(nb),
                     kBoundThreads, 0, st, p, T, strip, slots);
