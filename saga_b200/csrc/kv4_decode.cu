@@ -8,7 +8,8 @@
 //
 // Work: an item is a (request, key head, up to 16 of its query heads). Its
 // positions are tiles of 32; the tiles of all items form one list, of which
-// every CTA takes an equal run (lengths are read on the device). A warp works
+// every CTA takes an equal run (lengths are read on the device), where an item
+// counts for some tiles more than it has, since a CTA pays for each. A warp works
 // alone: it copies its next tiles into a ring of its own with one bulk copy per
 // head, and holds a running maximum, sums and outputs in registers. The warps
 // of a CTA meet at the end of an item; items cut by CTA borders leave partial
@@ -38,6 +39,11 @@ constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kMaxSlots = 16;       // query heads of an item
 constexpr int kMaxRing = 4;         // stages of a warp's ring
 constexpr int kMinTiles = 4;        // tiles of a CTA's run, at least: one warp per scheduler
+// Tiles that an item's own cost counts for when the work is dealt out: the start of its copies and the meeting
+// of the warps take about 5 us, a round of eight tiles 2 to 3 us. Sixteen ragged rows of up to 16,512 positions
+// take 19.0 us with 0, 15.8 with 8, 15.6 with 16 and 15.5 with 32; 64 ragged rows of up to 2048 positions 24.8,
+// 18.2, 18.5 and 21.1.
+constexpr int kItemTiles = 16;
 constexpr int kRingBytes = 216 * 1024;  // of all warps; static shared memory has the rest
 constexpr float kHead = 12.f;     // log2 of the greatest weight where the stabiliser was last set
 constexpr float kLow = 2048.f;    // SPLIT: the second term of a weight is held this much greater
@@ -72,7 +78,7 @@ struct DecodePlan4 {
   int tpp_shift;   // log2 of the tiles per page
   float* part_o;   // [grid][2][slots][D] numerators of cut items
   float* part_ml;  // [grid][2][slots][2] their maxima and sums
-  long long* prefix;  // [rows + 1] tiles before a (request, key head) row
+  long long* prefix;  // [rows + 1] weight of the items before a (request, key head) row
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -167,6 +173,9 @@ __device__ __forceinline__ RowInfo row_info(const SagaKv4Args& a, int r) {
   return i;
 }
 
+// What an item of the row counts for when the work is dealt out: kItemTiles, then its tiles.
+__device__ __forceinline__ int item_weight(const RowInfo& i) { return i.tiles ? kItemTiles + i.tiles : 0; }
+
 // Quotient of numbers that are not negative; 32 bits where they fit, since a 64-bit division takes about a
 // hundred instructions.
 __device__ __forceinline__ long long divide(long long a, long long b) {
@@ -216,7 +225,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   // ---- this CTA's run of tiles: [run, run_end), and the row it begins in
   long long total = 0;
   if (rows > kDecThreads) {
-    for (int r = threadIdx.x; r < rows; r += kDecThreads) total += row_info(a, r).tiles;
+    for (int r = threadIdx.x; r < rows; r += kDecThreads) total += item_weight(row_info(a, r));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) scan_sm[warp] = total;
@@ -230,7 +239,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   const bool writes_prefix = blockIdx.x == 0;
   for (int r0 = 0; r0 < rows; r0 += kDecThreads) {
     const int r = r0 + threadIdx.x;
-    const long long t = r < rows ? (long long)row_info(a, r).tiles * p.groups : 0;
+    const long long t = r < rows ? (long long)item_weight(row_info(a, r)) * p.groups : 0;
     long long inc = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -279,18 +288,19 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   while (run < run_end) {
     // ---- the item: row, slot group, tiles [t0, t1) of the row
     RowInfo ri = row_info(a, row);
-    while (run >= row_base + (long long)ri.tiles * p.groups) {
-      row_base += (long long)ri.tiles * p.groups;
+    while (run >= row_base + (long long)item_weight(ri) * p.groups) {
+      row_base += (long long)item_weight(ri) * p.groups;
       ri = row_info(a, ++row);
     }
     int sg = 0;
-    long long item_base = row_base;
-    while (run >= item_base + ri.tiles) {
-      item_base += ri.tiles;
+    long long tile_base = row_base + kItemTiles;  // of the item's tile 0
+    while (run >= tile_base + ri.tiles) {
+      tile_base += item_weight(ri);
       ++sg;
     }
-    const int t0 = (int)(run - item_base);
-    const int t1 = (int)min((long long)ri.tiles, run_end - item_base);
+    const int t0 = (int)max(run - tile_base, 0ll);
+    const int t1 = (int)min((long long)ri.tiles, run_end - tile_base);
+    if (t1 <= t0) break;  // the run ends before the item's first tile
     const int b = row / Hk, kh = row - b * Hk;
     const SlotGroup grp = slot_group(kh, sg, G, Gv, SLOTS, p.vheads);
     const int vh0 = grp.h0 / Gv;
@@ -818,7 +828,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     }
     fence_proxy_async_smem();  // the ring is written by bulk copies again
     __syncthreads();
-    run = item_base + t1;
+    run = tile_base + t1;
   }
 }
 
@@ -842,14 +852,14 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_combine_kernel(const DecodePla
   pdl_wait();
   if (threadIdx.x == 0 && a.lens[b] > a.max_pages * a.pool.page_len) set_status(a.status, SAGA_STATUS_PAGE_RANGE);
   const long long total = p.prefix[a.B * a.pool.Hk], first = p.prefix[row];
-  const long long tiles = divide(p.prefix[row + 1] - first, p.groups);
+  const long long weight = divide(p.prefix[row + 1] - first, p.groups);
   const int64_t at = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
-  if (tiles == 0) {
+  if (weight == 0) {
     for (int c = threadIdx.x; c < D; c += 32 * WARPS) store_out(a.out, a.dtype, at + c, 0.f);
     return;
   }
   const long long per = tiles_per_cta(total, grid);
-  const long long begin = first + sg * tiles, end = begin + tiles;
+  const long long begin = first + sg * weight + kItemTiles, end = first + (sg + 1) * weight;
   const int c0 = (int)divide(begin, per), n = (int)divide(end - 1, per) - c0 + 1;
   if (n == 1) return;  // one CTA had the whole item
   // part i: of CTA c0 + i; only the first part can begin with the item
