@@ -25,6 +25,15 @@
 //   output: A = codes transposed (ldmatrix.trans: channels x positions),
 //           B = weights (positions x slots): the scores' accumulators have
 //           exactly this layout, so the weights never leave their lane.
+//
+// Measured (with the join): 64 x 65,600 positions, 12 query, 1 key and 4 value
+// heads of 128, 338 us for 1.51 GB, 4.5 TB/s; 8 x 32,768, 12/1/2 heads, 26.6 us
+// for 56.6 MB, 2.1 TB/s. What bounds it is not the memory but the work per code:
+// the schedulers issue in 43 % of the cycles and the logical operations take 34 %
+// of theirs, and with 242 registers a thread there are two warps per scheduler to
+// cover the products' latency. Twelve warps spill and gain nothing; scores in
+// e4m3, whose instruction is twice as fast, need a further term per query and
+// its registers (31 us instead of 27).
 #include <algorithm>
 
 #include "kv4.cuh"
