@@ -9,58 +9,54 @@ namespace saga {
 
 namespace {
 
-// Four lanes hold one group: lane l has its values 8l .. 8l + 7 and 32 + 8l ..
-// 39 + 8l, so that 16-bit values arrive in 16-byte loads of 64 consecutive bytes
-// per group and leave as two words of codes per lane, 32 consecutive bytes (one
-// sector) per group. What is done once per group (the address, the scale) costs
-// as much as ten values, so fewer lanes with more values each are cheaper: eight
-// lanes of eight values took 98 us where these take 51 us (131,072 tokens, five
-// heads of 128, bf16: 215 MB, 4.2 TB/s). The write is bound by its instructions
-// (the schedulers issue in 83 % of the cycles), the read, 40 us, by its stores
-// (5.4 TB/s). The rows go past the caches (__ldcs, __stcs): a prompt's rows are
-// larger than L2, and the read took 43 us without.
-constexpr int kLanes = 4;
-constexpr int kCtaThreads = 256;
+// Two lanes hold one group, every second 16 bytes of its values each, so that
+// loads and stores take whole sectors; they exchange codes so that each leaves
+// (or reads) one of the group's two 16-byte chunks. What is done once per group (the
+// address, the scale) costs as much as ten values, so fewer lanes with more values
+// each are cheaper: 131,072 tokens of five heads of 128 in bf16 (215 MB) are written
+// in 98 us by eight lanes, 51 us by four (whose schedulers issue in 83 % of the cycles)
+// and 39.5 us by two, 5.4 TB/s; read in 39.6 us by four and 36.4 us by two, 5.9 TB/s.
+// The rows go past the caches (__ldcs, __stcs): a prompt's rows are larger than L2, and
+// the read took 3 us more without. CTAs of 256 threads write the same in 43.4 us, of 64 in 40.
+constexpr int kLanes = 2;
+constexpr int kVals = 64 / kLanes;
+constexpr int kCtaThreads = 128;
 constexpr int kCtaGroups = kCtaThreads / kLanes;
 constexpr int kAhead = 2;  // groups that a lane loads before it works on the first
 
-// Sixteen values of a lane as they are loaded.
+// A lane's values as they are loaded: every second 16 bytes of the group.
 template <typename T>
 struct Raw {
-  uint4 w[sizeof(T)];
+  uint4 w[kVals * sizeof(T) / 16];
 };
+template <typename T>
+constexpr int kPiece = 16 / sizeof(T);  // values of one load
 template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* p, Raw<T>& r) {
+__device__ __forceinline__ void load_vals(const T* p, Raw<T>& r) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < kVals / kPiece<T>; ++h) {
     if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        r.w[h * sizeof(T) / 2 + i] = __ldcs(reinterpret_cast<const uint4*>(p + 32 * h) + i);
+      r.w[h] = __ldcs(reinterpret_cast<const uint4*>(p + kLanes * kPiece<T> * h));
     } else {
-      T* t = reinterpret_cast<T*>(&r) + 8 * h;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = p[32 * h + i];
+      for (int i = 0; i < kPiece<T>; ++i) reinterpret_cast<T*>(&r.w[h])[i] = p[kLanes * kPiece<T> * h + i];
     }
   }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store16(T* p, const Raw<T>& r) {
+__device__ __forceinline__ void store_vals(T* p, const Raw<T>& r) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < kVals / kPiece<T>; ++h) {
     if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        __stcs(reinterpret_cast<uint4*>(p + 32 * h) + i, r.w[h * sizeof(T) / 2 + i]);
+      __stcs(reinterpret_cast<uint4*>(p + kLanes * kPiece<T> * h), r.w[h]);
     } else {
-      const T* t = reinterpret_cast<const T*>(&r) + 8 * h;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[32 * h + i] = t[i];
+      for (int i = 0; i < kPiece<T>; ++i) p[kLanes * kPiece<T> * h + i] = reinterpret_cast<const T*>(&r.w[h])[i];
     }
   }
 }
 
-// Least and greatest of a lane's sixteen values, and a value that is not 0 if
+// Least and greatest of a lane's values, and a value that is not 0 if
 // one of them is NaN or infinite. The 16-bit types are compared in pairs.
 template <typename T>
 __device__ __forceinline__ void extremes(const Raw<T>& r, float& lo, float& hi, float& odd) {
@@ -69,7 +65,7 @@ __device__ __forceinline__ void extremes(const Raw<T>& r, float& lo, float& hi, 
     lo = hi = x[0];
     odd = x[0] * 0.f;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) {
+    for (int i = 1; i < kVals; ++i) {
       lo = fminf(lo, x[i]);
       hi = fmaxf(hi, x[i]);
       odd = fmaf(x[i], 0.f, odd);
@@ -81,7 +77,7 @@ __device__ __forceinline__ void extremes(const Raw<T>& r, float& lo, float& hi, 
     *reinterpret_cast<uint32_t*>(&zero) = 0u;
     T2 a = x[0], b = x[0], o = __hmul2(x[0], zero);
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 1; i < kVals / 2; ++i) {
       a = __hmin2(a, x[i]);
       b = __hmax2(b, x[i]);
       o = __hfma2(x[i], zero, o);
@@ -118,7 +114,7 @@ struct Unit {
   bool is_v;
   bool live;  // the token exists
 };
-template <int D>
+template <int D, int PIECE>
 __device__ __forceinline__ Unit<D> locate_unit(uint32_t u, const Deal& d, const Rows& kr, const Rows& vr,
                                                const int64_t* __restrict__ slots, int l, int* status) {
   constexpr int NG = D / 64;
@@ -132,7 +128,7 @@ __device__ __forceinline__ Unit<D> locate_unit(uint32_t u, const Deal& d, const 
   int h = rest / NG;
   x.is_v = h >= kr.H;
   if (x.is_v) h -= kr.H;
-  x.src = t * (x.is_v ? vr.st : kr.st) + h * (x.is_v ? vr.sh : kr.sh) + x.g * 64 + l * 8;
+  x.src = t * (x.is_v ? vr.st : kr.st) + h * (x.is_v ? vr.sh : kr.sh) + x.g * 64 + l * PIECE;
   const bool inside = slot >= 0 && slot < d.slots;
   if (!inside && slot != -1 && rest == 0 && l == 0) set_status(status, SAGA_STATUS_PAGE_RANGE);
   x.row = (int)slot & (kKv4Tile - 1);
@@ -142,10 +138,38 @@ __device__ __forceinline__ Unit<D> locate_unit(uint32_t u, const Deal& d, const 
   x.tile = inside ? (x.is_v ? vr.pool : kr.pool) + tile * kv4_tile_bytes(D) : nullptr;
   return x;
 }
-// Where a lane's words of codes are: 8l .. 8l + 7 of the group in its first, 32 further in its second chunk.
+// w[h]: the codes of a lane's values 8h .. 8h + 7. In the tile lane l has chunk l,
+// so the two lanes exchange what the other needs. 16-bit types: w[h] is word 2h + l
+// of the group. fp32: its halves are those of words 2h and 2h + 1, the lower ones
+// in lane 0, the upper ones in lane 1.
+template <typename T>
+__device__ __forceinline__ uint4 chunk_of_codes(const uint32_t (&w)[4], int l) {
+  const uint32_t r0 = __shfl_xor_sync(0xffffffffu, l ? w[0] : w[2], 1);
+  const uint32_t r1 = __shfl_xor_sync(0xffffffffu, l ? w[1] : w[3], 1);
+  if constexpr (sizeof(T) == 2) return l ? make_uint4(r0, w[2], r1, w[3]) : make_uint4(w[0], r0, w[1], r1);
+  const uint32_t a0 = l ? r0 : w[0], a1 = l ? r1 : w[1], b0 = l ? w[2] : r0, b1 = l ? w[3] : r1;
+  return make_uint4(__byte_perm(a0, b0, 0x5410), __byte_perm(a0, b0, 0x7632), __byte_perm(a1, b1, 0x5410),
+                    __byte_perm(a1, b1, 0x7632));
+}
+template <typename T>
+__device__ __forceinline__ void codes_of_chunk(const uint4& c, int l, uint32_t (&w)[4]) {
+  uint32_t even[2] = {c.x, c.z}, odd[2] = {c.y, c.w};  // words of lane 0 and of lane 1
+  if constexpr (sizeof(T) == 4) {
+    even[0] = __byte_perm(c.x, c.y, 0x5410);
+    even[1] = __byte_perm(c.z, c.w, 0x5410);
+    odd[0] = __byte_perm(c.x, c.y, 0x7632);
+    odd[1] = __byte_perm(c.z, c.w, 0x7632);
+  }
+  const uint32_t r0 = __shfl_xor_sync(0xffffffffu, l ? even[0] : odd[0], 1);
+  const uint32_t r1 = __shfl_xor_sync(0xffffffffu, l ? even[1] : odd[1], 1);
+  w[0] = l ? r0 : even[0];
+  w[1] = l ? r1 : even[1];
+  w[2] = l ? odd[0] : r0;
+  w[3] = l ? odd[1] : r1;
+}
 template <int D>
-__device__ __forceinline__ uint32_t* code_word(const Unit<D>& x, int h, int l) {
-  return reinterpret_cast<uint32_t*>(x.tile + kv4_chunk_off<D>(x.row, x.g * 2 + h) + l * 4);
+__device__ __forceinline__ uint4* chunk_at(const Unit<D>& x, int l) {
+  return reinterpret_cast<uint4*>(x.tile + kv4_chunk_off<D>(x.row, x.g * 2 + l));
 }
 
 constexpr float kMagic = 8388608.f;  // 2^23: adding it rounds to a whole number, to nearest even
@@ -154,21 +178,22 @@ template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kCtaThreads) kv4_write_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                                 Rows kr, Rows vr, Deal deal,
                                                                 const int64_t* __restrict__ slots, int* status) {
+  constexpr int AHEAD = sizeof(T) == 4 ? 1 : kAhead;  // fp32: 32 registers a group (30.3 us, 32.2 us with two)
   pdl_wait();
   const int l = threadIdx.x & (kLanes - 1);
   const uint32_t units = (uint32_t)deal.strip * (uint32_t)deal.per;
-  const unsigned lanes = 0xfu << (threadIdx.x & 28);
-  for (uint32_t u0 = 0; u0 < units; u0 += kCtaGroups * kAhead) {  // the same trips for all lanes of a warp
-    Unit<D> at[kAhead];
-    Raw<T> raw[kAhead];
+  const unsigned lanes = 3u << (threadIdx.x & 30);
+  for (uint32_t u0 = 0; u0 < units; u0 += kCtaGroups * AHEAD) {  // the same trips for all lanes of a warp
+    Unit<D> at[AHEAD];
+    Raw<T> raw[AHEAD];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      at[i] = locate_unit<D>(u0 + i * kCtaGroups + threadIdx.x / kLanes, deal, kr, vr, slots, l, status);
+    for (int i = 0; i < AHEAD; ++i) {
+      at[i] = locate_unit<D, kPiece<T>>(u0 + i * kCtaGroups + threadIdx.x / kLanes, deal, kr, vr, slots, l, status);
       raw[i] = Raw<T>();
-      if (at[i].tile) load16<T, VEC>((at[i].is_v ? v : k) + at[i].src, raw[i]);
+      if (at[i].tile) load_vals<T, VEC>((at[i].is_v ? v : k) + at[i].src, raw[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {
       float lo, hi, odd;
       extremes<T>(raw[i], lo, hi, odd);
 #pragma unroll
@@ -189,19 +214,22 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_write_kernel(const T* __restr
       const f32x2 minus_z = pack2(-z, -z);
       constexpr uint32_t kOff = 0x4b000000u + (0x4b000000u << 4);  // the higher places overflow
       const T* x = reinterpret_cast<const T*>(&raw[i]);
+      uint32_t w[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w = 0;
+      for (int h = 0; h < 4; ++h) {
+        w[h] = 0;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           float y0, y1;
           unpack2(add2(pack2(Num<T>::to_f(x[8 * h + j]), Num<T>::to_f(x[8 * h + j + 1])), minus_z), y0, y1);
           // not packed: the assembler joins a packed product with the packed sum after it
-          w += __float_as_uint(__fadd_rn(__fmul_rn(y0, inv), kMagic)) << (4 * j);
-          w += __float_as_uint(__fadd_rn(__fmul_rn(y1, inv), kMagic)) << (4 * j + 4);
+          w[h] += __float_as_uint(__fadd_rn(__fmul_rn(y0, inv), kMagic)) << (4 * j);
+          w[h] += __float_as_uint(__fadd_rn(__fmul_rn(y1, inv), kMagic)) << (4 * j + 4);
         }
-        if (at[i].tile) *code_word<D>(at[i], h, l) = bad ? 0u : w - kOff;
+        w[h] = bad ? 0u : w[h] - kOff;
       }
+      const uint4 c = chunk_of_codes<T>(w, l);
+      if (at[i].tile) *chunk_at<D>(at[i], l) = c;
       if (l == 0 && at[i].tile) {
         const uint32_t m = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
         *reinterpret_cast<uint32_t*>(at[i].tile + kv4_meta_off<D>(at[i].row, at[i].g)) = bad ? 0x7fff7fffu : m;
@@ -233,19 +261,22 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
   const uint32_t units = (uint32_t)deal.strip * (uint32_t)deal.per;
   for (uint32_t u0 = 0; u0 < units; u0 += kCtaGroups * kAhead) {
     Unit<D> at[kAhead];
-    uint32_t w[kAhead][2], m[kAhead];
+    uint4 c[kAhead];
+    uint32_t m[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      at[i] = locate_unit<D>(u0 + i * kCtaGroups + threadIdx.x / kLanes, deal, kr, vr, slots, l, status);
-      w[i][0] = w[i][1] = m[i] = 0u;
+      at[i] = locate_unit<D, kPiece<T>>(u0 + i * kCtaGroups + threadIdx.x / kLanes, deal, kr, vr, slots, l, status);
+      c[i] = make_uint4(0u, 0u, 0u, 0u);
+      m[i] = 0u;
       if (at[i].tile) {
-        w[i][0] = *code_word<D>(at[i], 0, l);
-        w[i][1] = *code_word<D>(at[i], 1, l);
+        c[i] = *chunk_at<D>(at[i], l);
         m[i] = *reinterpret_cast<const uint32_t*>(at[i].tile + kv4_meta_off<D>(at[i].row, at[i].g));
       }
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
+      uint32_t w[4];
+      codes_of_chunk<T>(c[i], l, w);
       if (!at[i].live) continue;
       const float s = kv4_scale(m[i]), z = kv4_zero(m[i]);
       Raw<T> r;
@@ -253,9 +284,9 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
       const f32x2 s2 = pack2(s, s), z2 = pack2(z, z);
       // s * code has at most 12 significant bits, so the sum is rounded once
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 4; ++h) {
         f32x2 y[4];
-        codes8(w[i][h], y);
+        codes8(w[h], y);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float y0, y1;
@@ -264,7 +295,7 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
           x[8 * h + j + 4] = Num<T>::from_f(y1);
         }
       }
-      store16<T, VEC>((at[i].is_v ? v : k) + at[i].src, r);
+      store_vals<T, VEC>((at[i].is_v ? v : k) + at[i].src, r);
     }
   }
 }
@@ -372,12 +403,12 @@ void dispatch(int dt, int D, bool vec, F f) {
 
 }  // namespace
 
-// A CTA's strip is cut so that its groups fill all lanes kAhead deep about
-// twice, or to one token where there are too few tokens to fill the SMs so.
+// A CTA's strip is cut so that its groups fill all lanes kAhead deep, or to one
+// token where there are too few tokens to fill the SMs so.
 static int make_deal(const SagaKv4Pool& p, int64_t T, Deal* d, unsigned* grid) {
   d->T = T;
   d->per = (p.Hk + p.Hv) * (p.D / 64);
-  const int full = std::max(1, 2 * kAhead * kCtaGroups / d->per);
+  const int full = std::max(1, kAhead * kCtaGroups / d->per);
   d->strip = (int)std::max<int64_t>(1, std::min<int64_t>(full, T / (2 * 148)));
   // exact for u * per < 2^32; u stays below strip * per + 2 kAhead kCtaGroups
   d->magic = (uint32_t)(((1ull << 32) + d->per - 1) / d->per);
