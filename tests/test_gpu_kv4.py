@@ -139,6 +139,35 @@ def test_write_takes_strided_and_unaligned_rows():
         assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_unaligned_rows_of_every_type(dtype, d):
+    """Rows that start between 16-byte boundaries are written as aligned ones are, and read so by the C entry."""
+    from saga_b200 import _lib as L
+    from saga_b200 import kv4
+    T, hk, hv, pl = 300, 1, 2, 32
+    g = gen(3)
+    slots = torch.randperm(10 * pl, generator=g, device=DEV)[:T]
+    k, v = (torch.randn((T, h, d), generator=g, device=DEV).to(DT[dtype]) for h in (hk, hv))
+    wide = [torch.full((T, h, d + 3), 7.0, dtype=DT[dtype], device=DEV) for h in (hk, hv)]
+    for w, x in zip(wide, (k, v)):
+        w[:, :, 1:d + 1] = x
+    pools = [kv4.Kv4Pool(10, pl, hk, hv, d, device=DEV) for _ in range(2)]
+    kv4.kv4_write(pools[0], k, v, slots)
+    kv4.kv4_write(pools[1], wide[0][:, :, 1:d + 1], wide[1][:, :, 1:d + 1], slots)
+    assert torch.equal(pools[0].k, pools[1].k) and torch.equal(pools[0].v, pools[1].v)
+    want = kv4.kv4_read(pools[0], slots, DT[dtype])
+    at = [w[:, :, 1:d + 1] for w in wide]
+    rc = L.lib.saga_kv4_read(pools[0]._ref, {"bf16": L.SAGA_BF16, "fp16": L.SAGA_FP16, "fp32": L.SAGA_FP32}[dtype], T,
+                             slots.data_ptr(), at[0].data_ptr(), at[0].stride(0), at[0].stride(1), at[1].data_ptr(),
+                             at[1].stride(0), at[1].stride(1), None, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    for w, x in zip(wide, want):
+        assert torch.equal(w[:, :, 1:d + 1], x)
+        assert (w[:, :, 0] == 7).all() and (w[:, :, d + 1:] == 7).all()
+
+
 def test_one_value_for_all_heads_and_tokens():
     """Broadcast rows (zero strides)."""
     from saga_b200 import kv4
