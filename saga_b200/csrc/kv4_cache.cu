@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_read_kernel(T* __restrict__ k
 // `strip` tokens and takes the bounds of the pages that they complete. Threads
 // split a page into D/8 words of a row by 16 (32) rows. 1024 pages of 128 rows of
 // 128 take 10 us after the write that completes them (one page at a time and its
-// loads' latency: the schedulers issue in 38 % of the cycles); four rows of a
+// loads' latency: the schedulers issue in a third of the cycles); four rows of a
 // thread on their way together, since eight need 80 registers and leave fewer
 // CTAs per SM (13 us).
 constexpr int kBoundThreads = 256;
