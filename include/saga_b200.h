@@ -256,7 +256,7 @@ SAGA_API int saga_kv_append(int32_t dtype, int32_t B, int32_t Hk, int32_t Hv, in
  * bfloat16; s = (greatest - z) * (1/15), at least 2^-40, rounded up to
  * bfloat16; code = (x - z) * (1/s) rounded to nearest even, within 0..15. The
  * group stands for s * code + z. A group that holds a NaN or an infinity (or
- * whose s or z is not finite) stands for NaN.
+ * whose s or z is not finite) stands for NaN; it is held as s = 0, z = NaN.
  *
  * A pool holds num_pages pages of page_len positions. A position's slot is
  * page * page_len + offset. Pages are opaque to callers: [num_pages][H]

@@ -232,7 +232,9 @@ __global__ void __launch_bounds__(kCtaThreads) kv4_write_kernel(const T* __restr
       if (at[i].tile) *chunk_at<D>(at[i], l) = c;
       if (l == 0 && at[i].tile) {
         const uint32_t m = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
-        *reinterpret_cast<uint32_t*>(at[i].tile + kv4_meta_off<D>(at[i].row, at[i].g)) = bad ? 0x7fff7fffu : m;
+        // s = 0 and z = NaN for a group that is not finite: whatever the codes are, it stands for NaN, and the
+        // greatest scale of a row, which places the weights of the attention, is that of its other group
+        *reinterpret_cast<uint32_t*>(at[i].tile + kv4_meta_off<D>(at[i].row, at[i].g)) = bad ? 0x7fff0000u : m;
       }
     }
   }

@@ -1,0 +1,56 @@
+"""Attention over the 4-bit cache where the groups of a value row differ: a group of 64 values that stands for
+NaN beside one of numbers, and groups (or rows) whose scales lie far apart. What one group holds must not reach
+the others. Each group is compared with the 64-bit form of the channels of that group alone, so that a group of
+small values is held to a tolerance of its own.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4_oracle as O
+from test_gpu_kv4 import DEV, DT, OUT_EPS, W_EPS, Cache, _status, f32, f64, gen, slots_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def check_groups(q, out, k, v, scaling, dtype, nan=()):
+    """out [Hq, D] against the attention over k [n, Hk, D], v [n, Hv, D], group by group. nan: the
+    (value head, group) pairs that stand for NaN."""
+    q, out = f64(q), f64(out)
+    hq, hv = q.shape[0], v.shape[1]
+    ok = np.ones((k.shape[1], k.shape[0]), bool)
+    for g in range(q.shape[1] // 64):
+        only = np.zeros_like(v)
+        only[..., 64 * g:64 * g + 64] = v[..., 64 * g:64 * g + 64]
+        for vh, ng in nan:
+            if ng == g:
+                only[:, vh] = 0
+        ref, tol = O.attention(q, k, only, ok, scaling, W_EPS[dtype])
+        tol += OUT_EPS[dtype] * np.abs(ref) + 2.0 ** -25 * (dtype == "fp16")
+        for h in range(hq):
+            at = slice(64 * g, 64 * g + 64)
+            if (h // (hq // hv), g) in nan:
+                assert np.isnan(out[h, at]).all()
+            else:
+                err = np.abs(out[h, at] - ref[h, at])
+                assert (err <= tol[h, at]).all(), f"head {h}, group {g}: {err.max():.3e} over {tol[h, at].min():.3e}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("lens", [[256, 700], [20000, 9001]], ids=["one CTA", "cut"])
+def test_a_nan_value_group_stays_in_its_group(lens, what, dtype):
+    """One token of request 0 has a value group that is not finite; its keys are numbers."""
+    from saga_b200 import kv4
+    hq, hk, hv, d, pl, at = 12, 1, 4, 128, 128, 40
+    c = Cache(lens, hk, hv, d, pl, dtype, seed=21)
+    k = torch.randn((1, hk, d), generator=gen(1), device=DEV).to(DT[dtype])
+    v = torch.randn((1, hv, d), generator=gen(2), device=DEV).to(DT[dtype])
+    v[0, 1, 5] = float(what)      # the first group of value head 1
+    v[0, 2, 127] = float(what)    # the second of value head 2
+    kv4.kv4_write(c.pool, k, v, slots_of(c.table, 0, at + 1, pl, at))
+    c.k[0][at], c.v[0][at] = O.rows_value(f32(k))[0], O.rows_value(f32(v))[0]
+    q = torch.randn((2, hq, 1, d), generator=gen(3), device=DEV).to(DT[dtype])
+    out = kv4.kv4_decode(q, c.pool, c.table, c.device_lens)
+    check_groups(q[0, :, 0], out[0, :, 0], c.k[0], c.v[0], d ** -0.5, dtype, nan=[(1, 0), (2, 1)])
+    check_groups(q[1, :, 0], out[1, :, 0], c.k[1], c.v[1], d ** -0.5, dtype)
