@@ -54,7 +54,8 @@ constexpr int kMinTiles = 4;        // tiles of a CTA's run, at least: one warp 
 // 18.2, 18.5 and 21.1.
 constexpr int kItemTiles = 16;
 constexpr int kRingBytes = 216 * 1024;  // of all warps; static shared memory has the rest
-constexpr float kHead = 12.f;     // log2 of the greatest weight where the stabiliser was last set
+constexpr float kHead = 12.f;     // log2 of the greatest weight where the stabilisers were last set
+constexpr float kSlack = 15.f;    // log2 of the greatest weight, and of the greatest p, that is left as it is
 constexpr float kLow = 2048.f;    // SPLIT: the second term of a weight is held this much greater
 // -15, -16 * 15 and their sum in units of 2^-24, twice
 constexpr uint32_t kMinus15 = 0x800f800fu, kMinus240 = 0x80f080f0u, kMinus255 = 0x80ff80ffu;
@@ -135,9 +136,25 @@ __device__ __forceinline__ void mma16_first(float (&c)[4], uint32_t a0, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 // log2 of a positive bfloat16 scale, within 0.09 (its bits are a piecewise
-// linear logarithm). It only places the stabiliser of the weights.
+// linear logarithm). It only places the stabilisers.
 __device__ __forceinline__ float rough_log2(uint32_t bf16_bits) {
   return fmaf(__uint_as_float(0x4b000000u | bf16_bits), 0x1p-7f, -65663.f);
+}
+// The greatest of each over the four lanes of a quad.
+template <int N>
+__device__ __forceinline__ void quad_max(float (&x)[N]) {
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = __shfl_xor_sync(0xffffffffu, x[i], o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fmaxf(x[i], y[i]);
+  }
+}
+// 2^x of a whole number from -126 to 126: it is put where the exponent lies.
+__device__ __forceinline__ float exp2_whole(float x) {
+  return __uint_as_float(__float_as_uint(x + (12582912.f + 127.f)) << 23);
 }
 // 2 code - 15 (times 16 for the upper four bits of a byte), in units of 2^-24: exact in fp16.
 __device__ __forceinline__ uint32_t centre(uint32_t codes, uint32_t minus) {
@@ -469,7 +486,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     const uint32_t on_all = sh_on;
 
     f32x2 o[NT][D / 16][2];  // channel rows r8 and r8 + 8, two slots each
-    float mrun[NT];
+    float mrun[NT], shift[NT][NG];  // the stabilisers, whole numbers
     f32x2 lsum[NT], zsum[NT][NG];  // over the even and the odd positions
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -478,7 +495,10 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       mrun[i] = kNegInf;
       lsum[i] = 0ull;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) zsum[i][g] = 0ull;
+      for (int g = 0; g < NG; ++g) {
+        zsum[i][g] = 0ull;
+        shift[i][g] = 0.f;
+      }
     }
 
     for (int k = 0; k < mine; ++k) {
@@ -597,47 +617,84 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         }
       }
 
-      // ---- stabiliser, raised only when needed: weights p * s of at most 2^15 are left as they are.
-      // A new one puts a bound of the greatest weight at 2^kHead, so that weights far below it are still
-      // normal in fp16 (11 significant bits down to 2^-14). The bound joins the greatest score of a lane's
-      // positions and the greatest of their scales.
+      // ---- stabilisers. p = 2^(score - mrun) is of the scores alone; the weights p * s of group g are held
+      // 2^shift[g] times greater, so that a group of small values is as exact beside one of great values as by
+      // itself. Both are changed only when needed: p of at most 2^kSlack and weights of at most 2^kSlack are
+      // left as they are. Whether they are is asked of a bound, the greatest score of a lane's positions with
+      // the greatest of their scales.
       bool raise = false;
-      float mx[NT];
+      float top_l[NT];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const uint8_t* vm = kt + (1 + max(vhl[i], 0)) * TB + META;
-        uint32_t top = 0;
+        uint32_t top[NG];
         float y = kNegInf;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t vw[2][NG];
           load_meta<NG>(vm, 8 * j + 2 * c4, vw);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) top = max_u16x2(top, max_u16x2(vw[0][g], vw[1][g]));
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t t = max_u16x2(vw[0][g], vw[1][g]);
+            top[g] = j == 0 ? t : max_u16x2(top[g], t);
+          }
           float y0, y1;
           unpack2(l[i][j], y0, y1);
           y = fmaxf(y, fmaxf(y0, y1));
         }
-        y += rough_log2(top & 0xffffu);
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-        mx[i] = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-        raise |= mx[i] > mrun[i] + 15.f;
+        top_l[i] = y;
+        y -= mrun[i];
+        raise |= y > kSlack;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) raise |= y + shift[i][g] + rough_log2(top[g] & 0xffffu) > kSlack;
       }
       if (__any_sync(0xffffffffu, raise)) {
+        // New ones put the greatest score at or below 0 and the greatest weight, now position by position, at
+        // 2^kHead, so that weights far below it are still normal in fp16 (11 significant bits down to 2^-14).
+        // All are whole numbers: the factors between them are exact.
+        float down[NT], most[NT][NG];
+        quad_max(top_l);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          const float mn = fmaxf(mrun[i], mx[i] - kHead);
-          const float f = mn == kNegInf ? 1.f : ex2(mrun[i] - mn);
+          const float mn = fmaxf(mrun[i], ceilf(top_l[i]));
+          down[i] = mn == kNegInf ? 0.f : mrun[i] - mn;
           mrun[i] = mn;
+          const uint8_t* vm = kt + (1 + max(vhl[i], 0)) * TB + META;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) most[i][g] = kNegInf;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t vw[2][NG];
+            load_meta<NG>(vm, 8 * j + 2 * c4, vw);
+            float y0, y1;
+            unpack2(l[i][j], y0, y1);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+              most[i][g] = fmaxf(most[i][g], fmaxf(y0 - mn + rough_log2(vw[0][g] & 0xffffu),
+                                                   y1 - mn + rough_log2(vw[1][g] & 0xffffu)));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) quad_max(most[i]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const float f = ex2(down[i]);
           const f32x2 ff = pack2(f, f);
           lsum[i] = mul2(lsum[i], ff);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) zsum[i][g] = mul2(zsum[i][g], ff);
-          const f32x2 fo = pack2(__shfl_sync(0xffffffffu, f, 8 * c4), __shfl_sync(0xffffffffu, f, 8 * c4 + 4));
+          for (int g = 0; g < NG; ++g) {
+            zsum[i][g] = mul2(zsum[i][g], ff);
+            // a scale of 0 (a group that stands for NaN) leaves the shift within what 2^shift can be
+            const float to =
+                fmaxf(fminf(fminf(shift[i][g] - down[i], kHead - ceilf(most[i][g])), 126.f), -126.f);
+            const float fg = ex2(down[i] + (to - shift[i][g]));
+            shift[i][g] = to;
+            const f32x2 fo = pack2(__shfl_sync(0xffffffffu, fg, 8 * c4), __shfl_sync(0xffffffffu, fg, 8 * c4 + 4));
 #pragma unroll
-          for (int m = 0; m < D / 16; ++m) {
-            o[i][m][0] = mul2(o[i][m][0], fo);
-            o[i][m][1] = mul2(o[i][m][1], fo);
+            for (int m = 4 * g; m < 4 * g + 4; ++m) {
+              o[i][m][0] = mul2(o[i][m][0], fo);
+              o[i][m][1] = mul2(o[i][m][1], fo);
+            }
           }
         }
       }
@@ -663,8 +720,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
             // sum of p (z + 7.5 s): the products below take code - 7.5
             zsum[i][g] = fma2(pp, pack2(kv4_zero(vw[0][g]), kv4_zero(vw[1][g])), zsum[i][g]);
             zsum[i][g] = fma2(middle, w, zsum[i][g]);
+            const float up = exp2_whole(shift[i][g]);
             float w0, w1;
-            unpack2(w, w0, w1);
+            unpack2(mul2(w, pack2(up, up)), w0, w1);
             uint32_t& hi = wb[j >> 1][0][i][g][j & 1];
             hi = pack_half2(w0, w1);
             if constexpr (SPLIT) {
@@ -760,11 +818,14 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         sm_l[warp][r8 + 8 * i] = ls;
       }
       // slots 2 c4 and 2 c4 + 1 of the tile are this lane's columns
-      float z0[NG], z1[NG];
+      float z0[NG], z1[NG], u0[NG], u1[NG];  // offsets' sums; 2^-shift
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         z0[g] = __shfl_sync(0xffffffffu, lz[g], 8 * c4);
         z1[g] = __shfl_sync(0xffffffffu, lz[g], 8 * c4 + 4);
+        const float u = exp2_whole(-shift[i][g]);
+        u0[g] = __shfl_sync(0xffffffffu, u, 8 * c4);
+        u1[g] = __shfl_sync(0xffffffffu, u, 8 * c4 + 4);
       }
       if (mine > 0) {
 #pragma unroll
@@ -780,9 +841,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
           }
           float* s0 = so + (8 * i + 2 * c4) * RP + d;
           *reinterpret_cast<float2*>(s0) =
-              make_float2(fmaf(e0, 0x1p23f, z0[m / 4]), fmaf(h0, 0x1p19f, z0[m / 4]));
+              make_float2(fmaf(e0 * 0x1p23f, u0[m / 4], z0[m / 4]), fmaf(h0 * 0x1p19f, u0[m / 4], z0[m / 4]));
           *reinterpret_cast<float2*>(s0 + RP) =
-              make_float2(fmaf(e1, 0x1p23f, z1[m / 4]), fmaf(h1, 0x1p19f, z1[m / 4]));
+              make_float2(fmaf(e1 * 0x1p23f, u1[m / 4], z1[m / 4]), fmaf(h1 * 0x1p19f, u1[m / 4], z1[m / 4]));
         }
       }
     }

@@ -54,3 +54,62 @@ def test_a_nan_value_group_stays_in_its_group(lens, what, dtype):
     out = kv4.kv4_decode(q, c.pool, c.table, c.device_lens)
     check_groups(q[0, :, 0], out[0, :, 0], c.k[0], c.v[0], d ** -0.5, dtype, nan=[(1, 0), (2, 1)])
     check_groups(q[1, :, 0], out[1, :, 0], c.k[1], c.v[1], d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype,ratio", [("bf16", 1e8), ("bf16", 1e12), ("bf16", 1e30), ("fp32", 1e8), ("fp32", 1e12),
+                                         ("fp32", 1e30), ("fp16", 1e8)])
+@pytest.mark.parametrize("great", [0, 1])
+@pytest.mark.parametrize("lens", [[300], [20000]], ids=["one CTA", "cut"])
+def test_groups_of_values_far_apart(lens, great, dtype, ratio):
+    """One group of every value row is `ratio` times greater than the other."""
+    from saga_b200 import kv4
+    hq, hk, hv, d, pl, n = 12, 1, 2, 128, 128, lens[0]
+    c = Cache(lens, hk, hv, d, pl, dtype, seed=31)
+    v = torch.randn((n, hv, d), generator=gen(4), device=DEV)
+    v[..., 64 * great:64 * great + 64] *= ratio ** 0.5
+    v[..., 64 - 64 * great:128 - 64 * great] *= ratio ** -0.5
+    v = v.to(DT[dtype])
+    k = torch.randn((n, hk, d), generator=gen(5), device=DEV).to(DT[dtype])
+    kv4.kv4_write(c.pool, k, v, slots_of(c.table, 0, n, pl))
+    q = torch.randn((1, hq, 1, d), generator=gen(6), device=DEV).to(DT[dtype])
+    out = kv4.kv4_decode(q, c.pool, c.table, c.device_lens)
+    check_groups(q[0, :, 0], out[0, :, 0], O.rows_value(f32(k)), O.rows_value(f32(v)), d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [0, 3, 40, 600])
+def test_rows_of_values_far_apart(at, d, dtype):
+    """A row 10^12 times greater than the others whose weight is below 2^-90 of theirs: it adds less than 2^-48
+    of a value, so the attention over the other rows is what the result is compared with."""
+    from saga_b200 import kv4
+    n, pl = 700, 64
+    c = Cache([n], 1, 1, d, pl, dtype, seed=41)
+    q = torch.randn((1, 2, 1, d), generator=gen(7), device=DEV)
+    q[:, 1] = q[:, 0] * 0.9
+    q = q.to(DT[dtype])
+    k = torch.randn((n, 1, d), generator=gen(8), device=DEV) * 0.1
+    q0 = q[0, 0, 0].float()
+    k[at, 0] = -q0 * (90.0 * d ** 0.5 / float(q0 @ q0))        # scores of -90 and -81: e^-81 = 2^-116
+    v = torch.randn((n, 1, d), generator=gen(9), device=DEV)
+    v[at] *= 1e12
+    k, v = k.to(DT[dtype]), v.to(DT[dtype])
+    kv4.kv4_write(c.pool, k, v, slots_of(c.table, 0, n, pl))
+    out = kv4.kv4_decode(q, c.pool, c.table, c.device_lens)
+    others = [i for i in range(n) if i != at]
+    check_groups(q[0, :, 0], out[0, :, 0], O.rows_value(f32(k))[others], O.rows_value(f32(v))[others], d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", [1e-30, 1.0, 1e20, 1e30, -1e30])
+def test_value_rows_of_one_value(size, dtype):
+    """Constant rows have the least scale, 2^-40, beside an offset of any size."""
+    from saga_b200 import kv4
+    n, d, pl = 200, 128, 64
+    c = Cache([n], 1, 2, d, pl, dtype, seed=51)
+    v = torch.full((n, 2, d), size, device=DEV).to(DT[dtype])
+    k = torch.randn((n, 1, d), generator=gen(10), device=DEV).to(DT[dtype])
+    kv4.kv4_write(c.pool, k, v, slots_of(c.table, 0, n, pl))
+    q = torch.randn((1, 4, 1, d), generator=gen(11), device=DEV).to(DT[dtype])
+    out = kv4.kv4_decode(q, c.pool, c.table, c.device_lens)
+    check_groups(q[0, :, 0], out[0, :, 0], O.rows_value(f32(k)), O.rows_value(f32(v)), d ** -0.5, dtype)
