@@ -507,7 +507,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         cp0 = cp1;
         cp1 = ps1;  // `issue` has moved on to the batch after this one, if there is one
       }
-      if (!mbar_wait(&full[warp][st_c], par_c, a.status)) {
+      // the lanes vote: a copy that arrives near the limit must not leave some of them behind
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][st_c], par_c, a.status))) {
         // the copies in flight get one more bounded wait each; then this warp only keeps the barriers
         for (int x = k; x < min(k + p.stages, mine); ++x) {
           mbar_wait(&full[warp][st_c], par_c, a.status);
@@ -516,6 +517,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
             par_c ^= 1u;
           }
         }
+        __syncwarp();
         alive = false;
         break;
       }
@@ -798,6 +800,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     }
 
     // ---- the warps meet: numerators [slot][d] of each warp in its own ring
+    const int busy = min(t1 - t0, kDecWarps);  // warps that had tiles, or would have had before they gave up a wait
     float* so = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -827,7 +830,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
         u0[g] = __shfl_sync(0xffffffffu, u, 8 * c4);
         u1[g] = __shfl_sync(0xffffffffu, u, 8 * c4 + 4);
       }
-      if (mine > 0) {
+      if (warp < busy) {
 #pragma unroll
         for (int m = 0; m < D / 16; ++m) {
           // rows r8: channel d (kPairs: plus 16 times channel d + 1); rows r8 + 8: 16 times channel d + 1
@@ -848,7 +851,6 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       }
     }
     __syncthreads();
-    const int busy = min(t1 - t0, kDecWarps);  // warps that had tiles
     if (threadIdx.x < kDecWarps * SLOTS) {
       const int w = threadIdx.x / SLOTS, s = threadIdx.x % SLOTS;
       float M = kNegInf;
