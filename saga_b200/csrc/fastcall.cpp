@@ -42,7 +42,8 @@ struct Pool {
 };
 
 // A workspace for one call on the current stream: one is kept per (device,
-// stream), since calls in a stream do not overlap. A call under capture gets one
+// stream): a call makes all its launches before another thread can make one here,
+// since it holds Python's lock throughout. A call under capture gets one
 // of its own from the graph's memory: graphs captured on one stream may be
 // replayed on several. The kernels do not care what a workspace holds.
 std::map<std::pair<int, cudaStream_t>, at::Tensor>& scratches() {
@@ -145,16 +146,6 @@ PyObject* py_pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pool* p = new Pool{*reinterpret_cast<const SagaKv4Pool*>(desc), index, reinterpret_cast<int32_t*>(status), {}};
   return PyCapsule_New(p, "saga_kv4_pool",
                        [](PyObject* c) { delete reinterpret_cast<Pool*>(PyCapsule_GetPointer(c, "saga_kv4_pool")); });
-}
-
-// scratch(device index, stream, bytes): a workspace, to be held until the call has been made
-PyObject* py_scratch(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 3) return PyErr_Format(PyExc_TypeError, "scratch takes three arguments");
-  const int index = (int)PyLong_AsLong(a[0]);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(PyLong_AsVoidPtr(a[1]));
-  const size_t bytes = PyLong_AsSize_t(a[2]);
-  if (PyErr_Occurred()) return nullptr;
-  return guarded([&] { return THPVariable_Wrap(scratch(index, st, bytes)); });
 }
 
 // write(pool, k, v, slots) -> True
@@ -372,7 +363,7 @@ PyObject* py_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define METHOD(name) \
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_##name)), METH_FASTCALL, nullptr }
-PyMethodDef methods[] = {METHOD(bind), METHOD(pool), METHOD(scratch), METHOD(write), METHOD(read), METHOD(decode),
+PyMethodDef methods[] = {METHOD(bind), METHOD(pool), METHOD(write), METHOD(read), METHOD(decode),
                          METHOD(select), METHOD(tables), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

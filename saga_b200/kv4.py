@@ -269,6 +269,12 @@ def _kv4_args(q, pool: Kv4Pool, page_table, lens) -> L.SagaKv4Args:
     return a
 
 
+def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """A workspace for one call. Not one that is kept: ctypes lets other threads run during a call, whose launches
+    on the same stream may come between this call's."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
 def _kv4_run(fn, name: str, a: L.SagaKv4Args, op: int, pool: Kv4Pool) -> None:
     index = pool._index
     with _on_device(index):
@@ -276,11 +282,10 @@ def _kv4_run(fn, name: str, a: L.SagaKv4Args, op: int, pool: Kv4Pool) -> None:
         nbytes = L.lib.saga_kv4_workspace_bytes(ref, op)
         if nbytes == 0:
             raise L.SagaError(L.SAGA_ERR_INVALID, "saga_kv4_workspace_bytes")
-        stream = _raw_stream(index)
-        workspace = _fast.scratch(index, stream, nbytes)
+        workspace = _workspace(nbytes, pool.device)
         a.workspace = workspace.data_ptr()
         a.workspace_bytes = nbytes
-        rc = fn(ref, stream)
+        rc = fn(ref, _raw_stream(index))
     if rc:
         L.check(rc, name)
 
@@ -430,11 +435,10 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     a.status = _status(index)
     nbytes = max(16 * B, 16)
     with _on_device(index):
-        stream = _raw_stream(index)
-        workspace = _fast.scratch(index, stream, nbytes)
+        workspace = _workspace(nbytes, dev)
         a.workspace = workspace.data_ptr()
         a.workspace_bytes = nbytes
-        rc = L.lib.saga_page_tables(ctypes.byref(a), stream)
+        rc = L.lib.saga_page_tables(ctypes.byref(a), _raw_stream(index))
     if rc:
         L.check(rc, "saga_page_tables")
     return PageStep(slots, positions, offsets, lens_out, free_state_out)
