@@ -193,6 +193,7 @@ def kv4_write(pool: Kv4Pool, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
         return torch.ops.saga.kv4_write(*_tensors(pool), k, v, slots)
     if _fast.write(pool._handle, k, v, slots):
         return
+    k, v = k.resolve_neg(), v.resolve_neg()
     T = _rows(pool, k, v, slots)
     ks, vs = k.stride(), v.stride()
     with _on_device(pool._index):
@@ -306,6 +307,7 @@ def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     out = _fast.decode(pool._handle, query, page_table, lens, scaling, starts, blocks, counts)
     if out is not None:
         return out
+    query = query.resolve_neg()
     a = _kv4_args(query, pool, page_table, lens)
     B, Hq, D = a.B, a.Hq, pool.head_dim
     a.scaling = D ** -0.5 if scaling is None else float(scaling)
@@ -348,6 +350,7 @@ def kv4_select(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
         got = _fast.select(pool._handle, query, page_table, lens, top, keep_first, keep_last)
         if got is not None:
             return got
+    query = query.resolve_neg()
     a = _kv4_args(query, pool, page_table, lens)
     if pool.k_lo is None:
         raise ValueError("kv4_select needs a pool with bounds=True")

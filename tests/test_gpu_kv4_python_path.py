@@ -106,3 +106,24 @@ def test_threads_on_one_stream():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_the_negative_bit_is_not_ignored(dtype):
+    """A view whose sign is only noted on the tensor (as of a conjugate's imaginary part) stands for its values."""
+    from saga_b200 import kv4
+    c = Cache([200, 90], 1, 2, 64, 32, "fp32", seed=68, bounds=True)
+    q = queries(c, 8, dtype=dtype)
+    neg = torch._neg_view(-q)
+    assert neg.is_neg() and torch.equal(neg, q)
+    assert torch.equal(kv4.kv4_decode(neg, c.pool, c.table, c.device_lens),
+                       kv4.kv4_decode(q, c.pool, c.table, c.device_lens))
+    for a, b in zip(kv4.kv4_select(neg, c.pool, c.table, c.device_lens, 3),
+                    kv4.kv4_select(q, c.pool, c.table, c.device_lens, 3)):
+        assert torch.equal(a, b)
+    k, v = (torch.randn((40, h, 64), generator=gen(h), device=DEV).to(dtype) for h in (1, 2))
+    slots = torch.arange(40, device=DEV)
+    pools = [kv4.Kv4Pool(2, 32, 1, 2, 64, device=DEV) for _ in range(2)]
+    kv4.kv4_write(pools[0], k, v, slots)
+    kv4.kv4_write(pools[1], torch._neg_view(-k), torch._neg_view(-v), slots)
+    assert torch.equal(pools[0].k, pools[1].k) and torch.equal(pools[0].v, pools[1].v)
