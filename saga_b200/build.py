@@ -5,8 +5,9 @@
 Sources: saga_b200/csrc/*.cu. Output: saga_b200/libsaga_b200.so. The library
 links the CUDA runtime statically and has no PyTorch dependency. The host calls
 of the 4-bit cache operators (saga_b200/csrc/fastcall.cpp) are a CPython module
-of their own, saga_b200/_fastcall.so, which knows torch and is bound to the
-library at run time.
+of their own, saga_b200/_fastcall.<ABI tag>.so, which knows torch and is bound to
+the library at run time. It is built where torch is installed, and again after
+a change of torch, Python or the compiler; callers of the C ABI alone do without.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -24,7 +26,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsaga_b200.so")
 STAMP = os.path.join(HERE, ".libsaga_b200.stamp")
 FAST_SRC = os.path.join(CSRC, "fastcall.cpp")
-FAST = os.path.join(HERE, "_fastcall.so")
+FAST = os.path.join(HERE, "_fastcall" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -55,22 +57,34 @@ def _digest() -> str:
             h.update(os.path.basename(f).encode())
             h.update(fh.read())
     h.update(" ".join(ARCH + FLAGS).encode())
+    fast = _fast_command(FAST)
+    if fast:  # what the call module takes from torch's headers and Python's depends on their versions
+        import torch
+        h.update(" ".join([*fast, torch.__version__, sys.version]).encode())
     return h.hexdigest()
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(FAST) or not os.path.exists(STAMP):
-        return False
+def _stamped() -> str:
+    """What the built files were made of, or nothing."""
+    if not os.path.exists(STAMP):
+        return ""
     with open(STAMP) as f:
-        return f.read().strip() == _digest()
+        return f.read().strip()
 
 
-def _fast_command(out: str) -> list:
-    """The g++ command of the torch-facing call module."""
-    import sysconfig
+def up_to_date() -> bool:
+    if not os.path.exists(LIB) or (_fast_command(FAST) and not os.path.exists(FAST)):
+        return False
+    return _stamped() == _digest()
 
-    import torch
-    from torch.utils.cpp_extension import include_paths, library_paths
+
+def _fast_command(out: str):
+    """The g++ command of the torch-facing call module, or None without torch."""
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths, library_paths
+    except ImportError:
+        return None
 
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
@@ -98,8 +112,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd = [nvcc, *ARCH, *FLAGS, "-I", os.path.join(REPO, "include"), "-dc" if False else "-c", src, "-o", obj]
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     fast_tmp = FAST + ".tmp"
-    procs.append((FAST_SRC, subprocess.Popen(_fast_command(fast_tmp), stdout=subprocess.PIPE,
-                                             stderr=subprocess.STDOUT, text=True)))
+    fast = _fast_command(fast_tmp)
+    if fast:
+        procs.append((FAST_SRC, subprocess.Popen(fast, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    else:
+        print("torch is not installed: the library for the C ABI alone is built")
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -108,7 +125,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if p.returncode:
             failed.append(src)
     if failed:
-        raise RuntimeError(f"nvcc failed for {failed}")
+        raise RuntimeError(f"compiling failed for {failed}")
     tmp = LIB + ".tmp"
     cmd = [nvcc, *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -116,7 +133,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         sys.stdout.write(r.stdout + r.stderr)
         raise RuntimeError("link failed")
     os.replace(tmp, LIB)
-    os.replace(fast_tmp, FAST)
+    if fast:
+        os.replace(fast_tmp, FAST)
     with open(STAMP, "w") as f:
         f.write(_digest())
     return LIB

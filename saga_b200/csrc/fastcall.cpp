@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/version.h>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -369,4 +370,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fastcall(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__fastcall(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION)) Py_CLEAR(m);
+  return m;
+}

@@ -19,6 +19,7 @@ batch (speedup.py:119-139).
 from __future__ import annotations
 
 import ctypes
+import re
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -29,8 +30,19 @@ from .ops import _DT, _STATUS, status_tensor
 try:
     from . import _fastcall as _fast  # after torch, whose libraries it uses
 except ImportError as e:
-    raise ImportError("saga_b200/_fastcall.so is missing or does not load: build it with "
-                      "`python -m saga_b200.build`") from e
+    raise ImportError("saga_b200/_fastcall is missing or does not load: build it with "
+                      "`python -m saga_b200.build --force`") from e
+
+
+def _check_built_for(module) -> None:
+    """Refuses a call module built against another torch, whose tensors may be laid out otherwise."""
+    built, have = getattr(module, "torch_version", None), re.match(r"\d+\.\d+\.\d+", torch.__version__).group()
+    if built != have:
+        raise ImportError(f"saga_b200/_fastcall was built for torch {built}, this is {have}: build it again with "
+                          "`python -m saga_b200.build --force`")
+
+
+_check_built_for(_fast)
 _fast.bind(*(ctypes.cast(getattr(L.lib, f), ctypes.c_void_p).value for f in
              ("saga_kv4_write", "saga_kv4_read", "saga_kv4_workspace_bytes", "saga_kv4_decode", "saga_kv4_select",
               "saga_page_tables")))
