@@ -464,6 +464,8 @@ def slot_map(page_table: torch.Tensor, lens: torch.Tensor, num_tokens: int, page
     """The slots (int64 [num_tokens]) of the positions [starts[b], lens[b]) that
     the requests already hold, packed in order of the requests, and their
     offsets (int32 [B + 1]). Rows beyond the last position get -1."""
+    if torch.compiler.is_compiling():
+        return torch.ops.saga.slot_map(page_table, lens, num_tokens, page_len, starts)
     if not page_table.is_cuda:
         _bad_cuda()
     index, dev = page_table.get_device(), page_table.device
@@ -558,3 +560,14 @@ def _op_page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torc
 def _(page_table, lens, new_lens, free_pages, free_state, num_tokens, page_len):
     return (lens.new_empty(num_tokens, dtype=torch.int64), lens.new_empty(num_tokens), lens.new_empty(lens.numel() + 1),
             torch.empty_like(lens), torch.empty_like(free_state))
+
+
+@torch.library.custom_op("saga::slot_map", mutates_args=())
+def _op_slot_map(page_table: torch.Tensor, lens: torch.Tensor, num_tokens: int, page_len: int,
+                 starts: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    return slot_map(page_table, lens, num_tokens, page_len, starts)
+
+
+@_op_slot_map.register_fake
+def _(page_table, lens, num_tokens, page_len, starts):
+    return lens.new_empty(num_tokens, dtype=torch.int64), lens.new_empty(lens.numel() + 1)
