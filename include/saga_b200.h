@@ -343,7 +343,8 @@ SAGA_API int saga_kv4_select(const SagaKv4Args* args, void* stream);
  * whose pages, table row or token rows do not suffice gets nothing: its tokens
  * get slot -1, its length stays and SAGA_STATUS_OUT_OF_PAGES is set. new_lens[b]
  * < 0 finishes request b: its pages go to the ring's end and its length becomes
- * 0. lens_out and free_state_out may be lens and free_state themselves. */
+ * 0. The ring has to have room for every page; a finished request whose pages
+ * find none keeps them and its length, and SAGA_STATUS_PAGE_RANGE is set. lens_out and free_state_out may be lens and free_state themselves. */
 typedef struct SagaPageTableArgs {
   int32_t B, page_len, max_pages;
   int32_t* page_table; int64_t pt_sb;             /* [B, max_pages], entries of new pages are written */

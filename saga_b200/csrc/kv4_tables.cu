@@ -61,8 +61,8 @@ __device__ __forceinline__ void scan(long long (&v)[N], long long (&tot)[N], lon
 
 __device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
   __shared__ long long sm[2][33];
-  __shared__ int taken_sm;
-  if (threadIdx.x == 0) taken_sm = 0;
+  __shared__ int taken_sm, returned_sm;
+  if (threadIdx.x == 0) taken_sm = returned_sm = 0;
   const int shift = __ffs(a.page_len) - 1;
   const long long cover = (long long)a.max_pages << shift;
   const int head = a.free_state[0];
@@ -83,26 +83,31 @@ __device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
     tok += tot1[0];
     const bool fits = end <= cover && start + add <= a.num_tokens;
     const int need = fits ? (int)(((end + a.page_len - 1) >> shift) - held) : 0;
-    const int back = in && raw < 0 && a.ring ? min(held, a.max_pages) : 0;
+    const int back = in && raw < 0 ? min(held, a.max_pages) : 0;
     long long v[2] = {need, back}, tot[2];
     scan(v, tot, sm);
     const long long upto = want + v[0] + need;
     const bool granted = fits && (need == 0 || upto <= count);
+    // pages go back to the entries that are not free, so nothing that is free is written over
     const long long before = ret + v[1];
+    const bool room = back == 0 || before + back <= a.ring - count;
     want += tot[0];
     ret += tot[1];
-    // the granted requests that need pages are the first ones that do, so the last one's sum is the total
+    // the granted requests that need pages are the first ones that do, so the last one's sum is the total; the
+    // same holds of the returned pages
     if (granted && need) atomicMax(&taken_sm, (int)upto);
+    if (room && back) atomicMax(&returned_sm, (int)(before + back));
     if (in) {
       TableRow r;
       r.len = granted ? len : -1;
       r.first = a.ring ? (int)((h0 + upto - need) % a.ring) : 0;
-      r.back = back ? (int)((h0 + (long long)count + before) % a.ring) : -1;
+      r.back = back && room ? (int)((h0 + (long long)count + before) % a.ring) : -1;
       r.held = held;
       rows[b] = r;
       a.offsets[b + 1] = (int)min(start + add, 0x7fffffffll);
-      a.lens_out[b] = raw < 0 ? 0 : granted ? (int)end : len;
+      a.lens_out[b] = raw < 0 ? (room ? 0 : len) : granted ? (int)end : len;
       if (!granted && add > 0) set_status(a.status, SAGA_STATUS_OUT_OF_PAGES);
+      if (!room) set_status(a.status, SAGA_STATUS_PAGE_RANGE);
     }
   }
   __syncthreads();
@@ -110,7 +115,7 @@ __device__ void table_scan(const SagaPageTableArgs& a, TableRow* rows) {
     const int taken = taken_sm;
     a.offsets[0] = 0;
     a.free_state_out[0] = a.ring ? (int)((h0 + taken) % a.ring) : 0;
-    a.free_state_out[1] = (int)(count - taken + ret);
+    a.free_state_out[1] = count - taken + returned_sm;
   }
 }
 

@@ -401,7 +401,8 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     place). A request that cannot be given all its pages, table entries or rows
     gets nothing: slots -1, its length unchanged, ``STATUS_OUT_OF_PAGES`` set.
     ``new_lens[b] < 0`` finishes request b: its pages return to the ring's end
-    and its length becomes 0.
+    and its length becomes 0 (in a ring without room for them it keeps both, and
+    ``STATUS_PAGE_RANGE`` is set).
 
     ``lens_out`` and ``free_state_out`` may be ``lens`` and ``free_state`` (an
     update in place, e.g. inside a CUDA graph); by default they are new tensors.
