@@ -239,16 +239,17 @@ def kv4_read(pool: Kv4Pool, slots: torch.Tensor, dtype: torch.dtype = torch.bflo
     return k, v
 
 
-def _table(t, index: int, B: int) -> int:
+def _table(t, index: int, B: int) -> Tuple[int, int]:
+    """Address and row stride of a page table. The stride of a dimension of one says nothing."""
     if t.dtype is not _I32:
         raise TypeError(f"page_table must be {_I32}")
     if not t.is_cuda:
         _bad_cuda()
     if t.get_device() != index:
         raise ValueError(f"page_table is on {t.device}, not on cuda:{index}")
-    if t.dim() != 2 or t.shape[0] < B or (t.stride(1) != 1 and t.numel()):
+    if t.dim() != 2 or t.shape[0] < B or (t.stride(1) != 1 and t.shape[1] > 1 and t.numel()):
         raise ValueError("page_table must be an int32 [B, max_pages] tensor with unit column stride")
-    return t.data_ptr()
+    return t.data_ptr(), t.shape[1] if t.shape[0] == 1 else t.stride(0)
 
 
 def _kv4_args(q, pool: Kv4Pool, page_table, lens) -> L.SagaKv4Args:
@@ -274,8 +275,7 @@ def _kv4_args(q, pool: Kv4Pool, page_table, lens) -> L.SagaKv4Args:
     a.q = q.data_ptr()
     a.q_sb = qs[0]
     a.q_sh = qs[1]
-    a.page_table = _table(page_table, index, B)
-    a.pt_sb = page_table.stride(0)
+    a.page_table, a.pt_sb = _table(page_table, index, B)
     a.max_pages = page_table.shape[1]
     a.lens = _ints("lens", lens, index, _I32, (B,))
     a.status = pool._status
@@ -429,8 +429,7 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     a = L.SagaPageTableArgs()
     a.B = B
     a.page_len = int(page_len)
-    a.page_table = _table(page_table, index, B)
-    a.pt_sb = page_table.stride(0)
+    a.page_table, a.pt_sb = _table(page_table, index, B)
     a.max_pages = page_table.shape[1]
     a.lens = _ints("lens", lens, index, _I32, (B,))
     a.new_lens = _ints("new_lens", new_lens, index, _I32, (B,))
@@ -471,7 +470,7 @@ def slot_map(page_table: torch.Tensor, lens: torch.Tensor, num_tokens: int, page
         _bad_cuda()
     index, dev = page_table.get_device(), page_table.device
     B = lens.numel()
-    table = _table(page_table, index, B)
+    table, row = _table(page_table, index, B)
     at = _ints("lens", lens, index, _I32, (B,))
     first = None if starts is None else _ints("starts", starts, index, _I32, (B,))
     num_tokens = int(num_tokens)
@@ -480,8 +479,8 @@ def slot_map(page_table: torch.Tensor, lens: torch.Tensor, num_tokens: int, page
     slots = torch.empty(num_tokens, dtype=_I64, device=dev)
     offsets = torch.empty(B + 1, dtype=_I32, device=dev)
     with _on_device(index):
-        rc = L.lib.saga_slot_map(B, int(page_len), table, page_table.stride(0), page_table.shape[1], first, at,
-                                 num_tokens, slots.data_ptr(), offsets.data_ptr(), _status(index), _raw_stream(index))
+        rc = L.lib.saga_slot_map(B, int(page_len), table, row, page_table.shape[1], first, at, num_tokens,
+                                  slots.data_ptr(), offsets.data_ptr(), _status(index), _raw_stream(index))
     if rc:
         L.check(rc, "saga_slot_map")
     return slots, offsets

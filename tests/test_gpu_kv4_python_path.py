@@ -127,3 +127,33 @@ def test_the_negative_bit_is_not_ignored(dtype):
     kv4.kv4_write(pools[0], k, v, slots)
     kv4.kv4_write(pools[1], torch._neg_view(-k), torch._neg_view(-v), slots)
     assert torch.equal(pools[0].k, pools[1].k) and torch.equal(pools[0].v, pools[1].v)
+
+
+def test_strides_of_dimensions_of_one():
+    """The stride of a table's only column, and of its only row, says nothing."""
+    from saga_b200 import kv4
+    c = Cache([200], 1, 2, 64, 32, seed=69, bounds=True)
+    q = queries(c, 8)
+    row = c.table.as_strided(c.table.shape, (1, 1))
+    assert row.stride(0) == 1 and row.shape[1] > 1
+    assert torch.equal(kv4.kv4_decode(q, c.pool, row, c.device_lens), kv4.kv4_decode(q, c.pool, c.table, c.device_lens))
+    for a, b in zip(kv4.kv4_select(q, c.pool, row, c.device_lens, 3), kv4.kv4_select(q, c.pool, c.table, c.device_lens, 3)):
+        assert torch.equal(a, b)
+    for a, b in zip(kv4.slot_map(row, c.device_lens, 200, 32), kv4.slot_map(c.table, c.device_lens, 200, 32)):
+        assert torch.equal(a, b)
+    c = Cache([20, 32, 5], 1, 2, 64, 32, seed=70)
+    q = queries(c, 8)
+    one = c.table[:, 0].contiguous()
+    column = one.view(1, 3).t()
+    assert column.stride() == (1, 3)
+    assert torch.equal(kv4.kv4_decode(q, c.pool, column, c.device_lens),
+                       kv4.kv4_decode(q, c.pool, one[:, None], c.device_lens))
+    i32 = dict(dtype=torch.int32, device=DEV)
+    tables = [torch.full((1, 3), -1, **i32).t(), torch.full((3, 1), -1, **i32)]
+    steps = [kv4.page_tables(t, torch.zeros(3, **i32), torch.tensor([5, 0, 32], **i32), torch.arange(9, **i32),
+                             torch.tensor([0, 9], **i32), 37, 32) for t in tables]
+    assert all(torch.equal(a, b) for a, b in zip(*steps)) and torch.equal(*tables)
+    tables = [torch.full((5, 1), -1, **i32).t(), torch.full((1, 5), -1, **i32)]
+    steps = [kv4.page_tables(t, torch.zeros(1, **i32), torch.tensor([100], **i32), torch.arange(9, **i32),
+                             torch.tensor([0, 9], **i32), 100, 32) for t in tables]
+    assert all(torch.equal(a, b) for a, b in zip(*steps)) and torch.equal(*tables)
