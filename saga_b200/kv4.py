@@ -102,7 +102,8 @@ class Kv4Pool:
 
     A position's slot is ``page * page_len + offset``. With ``bounds`` the pool
     also keeps the key bounds that ``kv4_select`` reads (``k_lo``, ``k_hi``:
-    bfloat16 ``[num_pages, key_heads, head_dim]``).
+    bfloat16 ``[num_pages, key_heads, head_dim]``). Its tensors can be written
+    to, but not exchanged: the calls know their addresses.
     """
 
     def __init__(self, num_pages: int, page_len: int, key_heads: int, value_heads: int, head_dim: int,
@@ -157,6 +158,14 @@ class Kv4Pool:
         self._ref = ctypes.byref(self._desc)
         self._status = _status(self._index)
         self._handle = _fast.pool(ctypes.addressof(self._desc), self._index, self._status)
+
+    def __setattr__(self, name, value):
+        if "_handle" in self.__dict__:
+            raise AttributeError(f"{name} of a Kv4Pool is fixed: Kv4Pool.of makes a pool of other tensors")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{name} of a Kv4Pool is fixed: Kv4Pool.of makes a pool of other tensors")
 
     def descriptor(self) -> L.SagaKv4Pool:
         """The C descriptor of the pool's tensors."""
