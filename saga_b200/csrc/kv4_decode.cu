@@ -57,8 +57,8 @@ constexpr int kRingBytes = 216 * 1024;  // of all warps; static shared memory ha
 constexpr float kHead = 12.f;     // log2 of the greatest weight where the stabilisers were last set
 constexpr float kSlack = 15.f;    // log2 of the greatest weight, and of the greatest p, that is left as it is
 constexpr float kLow = 2048.f;    // SPLIT: the second term of a weight is held this much greater
-// -15, -16 * 15 and their sum in units of 2^-24, twice
-constexpr uint32_t kMinus15 = 0x800f800fu, kMinus240 = 0x80f080f0u, kMinus255 = 0x80ff80ffu;
+// -16 * 15, and -15 with it, in units of 2^-24, twice
+constexpr uint32_t kMinus240 = 0x80f080f0u, kMinus255 = 0x80ff80ffu;
 constexpr float kNegInf = -INFINITY;
 
 // Query heads of a key head are cut into slot groups: consecutive heads, at most
@@ -156,10 +156,27 @@ __device__ __forceinline__ void quad_max(float (&x)[N]) {
 __device__ __forceinline__ float exp2_whole(float x) {
   return __uint_as_float(__float_as_uint(x + (12582912.f + 127.f)) << 23);
 }
-// 2 code - 15 (times 16 for the upper four bits of a byte), in units of 2^-24: exact in fp16.
+// 2 code - 15 of a byte's codes (the upper one's times 16), in units of 2^-24: exact in fp16.
 __device__ __forceinline__ uint32_t centre(uint32_t codes, uint32_t minus) {
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&codes), __floats2half2_rn(2.f, 2.f),
                             *reinterpret_cast<const __half2*>(&minus));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// SPLIT: codes as normal fp16 numbers (those of bits 0-3, or 16 times those of bits 4-7), and 32 code - 240 of bits
+// 4-7; set into the low bits of 1024 they are exact. The tensor cores align the products of a sum by the exponents
+// of their operands, a subnormal's being that of 2^-14: up to ten bits of a product with a code of 2^-24 are lost
+// beside the greatest query or weight. Terms of 22 bits feel that (fp32 errors 3 to 4e-6 with subnormals, 3 to 5e-7
+// without; 4 x 4099 positions 13.0 and 13.4 us), one term of 11 bits does not (fp16 3.0e-4 both ways, and 8 x 32,768
+// positions 29.3 and 29.8 us).
+__device__ __forceinline__ uint32_t whole(uint32_t codes) {
+  const uint32_t u = codes | 0x64006400u;
+  const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(-1024.f, -1024.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t centre16(uint32_t codes) {
+  const uint32_t u = codes | 0x64006400u;
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(2.f, 2.f),
+                            __floats2half2_rn(-2288.f, -2288.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 // The scale words of positions pos and pos + 1 (pos even).
@@ -212,7 +229,11 @@ __device__ __forceinline__ long long tiles_per_cta(long long total, int grid) {
 }
 
 // D: head_dim; NT: tiles of eight slots; SPLIT: queries and weights as two fp16
-// terms each (fp32 tensors, 22 significant bits).
+// terms each (fp32 tensors, 22 significant bits). bf16 and fp16 tensors take
+// weights of one fp16 term, which is a choice: its rounding is averaged over the
+// positions, and a second term would double the output's products. Relative rms
+// errors (and those of binary32 arithmetic rounded once): fp16 3.0e-4 (2.1e-4),
+// bf16 1.67e-3 (1.65e-3), fp32 3 to 5e-7 (5 to 15e-7).
 template <int D, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const DecodePlan4 p) {
   constexpr int NG = D / 64, CH = D / 32, NP = SPLIT ? 2 : 1, SLOTS = 8 * NT;
@@ -221,6 +242,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   // Whether channel rows 0-7 of a product take both codes of a byte, c + 16 c' (rows 8-15 have 16 c' and are
   // taken off at the end): an AND less per code, four bits less of the sums.
   constexpr bool kPairs = !SPLIT;
+  // what a product's one is, in channel rows 0-7 and 8-15
+  constexpr float kUnitE = SPLIT ? 0x1p-5f : 0x1p23f, kUnitH = SPLIT ? 0x1p-5f : 0x1p19f;
   constexpr int RP = D + 4;   // pitch of a warp's outputs when the warps meet
   constexpr int QP = D + 8;   // pitch of the queries
   constexpr int QT = 16, QC = D / QT;  // threads per slot's query, channels of each
@@ -479,7 +502,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       const int s = r8 + 8 * i;
       vhl[i] = slot_vh[s];
       const float unit = q_unit[s];
-      fh[i] = pack2(unit * 0x1p24f, unit * 0x1p24f);
+      fh[i] = pack2(unit * (SPLIT ? 1.f : 0x1p24f), unit * (SPLIT ? 1.f : 0x1p24f));
 #pragma unroll
       for (int g = 0; g < NG; ++g) Qz[i][g] = pack2(q_sum[s][g] * unit, q_sum[s][g] * unit);
     }
@@ -582,7 +605,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const uint32_t w = h ? kreg[j][ch] >> 8 : kreg[j][ch];
-                  const uint32_t x0 = w & 0x000f000fu, x1 = w & 0x00f000f0u;
+                  const uint32_t x0 = SPLIT ? whole(w & 0x000f000fu) : w & 0x000f000fu;
+                  const uint32_t x1 = SPLIT ? whole(w & 0x00f000f0u) : w & 0x00f000f0u;
                   const uint32_t a1 = NT == 2 ? q[NT - 1][2 * h] : 0u, a3 = NT == 2 ? q[NT - 1][2 * h + 1] : 0u;
                   if (ch == c0 && t == 0 && h == 0) mma16_first(acc[j], q[0][2 * h], a1, q[0][2 * h + 1], a3, x0, x1);
                   else mma16(acc[j], q[0][2 * h], a1, q[0][2 * h + 1], a3, x0, x1);
@@ -776,9 +800,18 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
                   // bytes y & 1 and 2 + (y & 1) as fp16: c + 16 c' of two positions
                   const uint32_t u0 = y & 1 ? __byte_perm(w0, 0, 0x4341) : w0 & 0x00ff00ffu;
                   const uint32_t u1 = y & 1 ? __byte_perm(w1, 0, 0x4341) : w1 & 0x00ff00ffu;
-                  const uint32_t a0 = centre(kPairs ? u0 : u0 & 0x000f000fu, kPairs ? kMinus255 : kMinus15),
-                                 a2 = centre(kPairs ? u1 : u1 & 0x000f000fu, kPairs ? kMinus255 : kMinus15),
-                                 a1 = centre(u0 & 0x00f000f0u, kMinus240), a3 = centre(u1 & 0x00f000f0u, kMinus240);
+                  uint32_t a0, a1, a2, a3;
+                  if constexpr (SPLIT) {
+                    a0 = centre16((u0 << 4) & 0x00f000f0u);
+                    a2 = centre16((u1 << 4) & 0x00f000f0u);
+                    a1 = centre16(u0 & 0x00f000f0u);
+                    a3 = centre16(u1 & 0x00f000f0u);
+                  } else {
+                    a0 = centre(u0, kMinus255);
+                    a2 = centre(u1, kMinus255);
+                    a1 = centre(u0 & 0x00f000f0u, kMinus240);
+                    a3 = centre(u1 & 0x00f000f0u, kMinus240);
+                  }
                   if (jj == 0) mma16_first(s[n][y], a0, a1, a2, a3, wv[g][jj][n][0], wv[g][jj][n][1]);
                   else mma16(s[n][y], a0, a1, a2, a3, wv[g][jj][n][0], wv[g][jj][n][1]);
                 }
@@ -844,9 +877,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
           }
           float* s0 = so + (8 * i + 2 * c4) * RP + d;
           *reinterpret_cast<float2*>(s0) =
-              make_float2(fmaf(e0 * 0x1p23f, u0[m / 4], z0[m / 4]), fmaf(h0 * 0x1p19f, u0[m / 4], z0[m / 4]));
+              make_float2(fmaf(e0 * kUnitE, u0[m / 4], z0[m / 4]), fmaf(h0 * kUnitH, u0[m / 4], z0[m / 4]));
           *reinterpret_cast<float2*>(s0 + RP) =
-              make_float2(fmaf(e1 * 0x1p23f, u1[m / 4], z1[m / 4]), fmaf(h1 * 0x1p19f, u1[m / 4], z1[m / 4]));
+              make_float2(fmaf(e1 * kUnitE, u1[m / 4], z1[m / 4]), fmaf(h1 * kUnitH, u1[m / 4], z1[m / 4]));
         }
       }
     }

@@ -113,3 +113,19 @@ def test_value_rows_of_one_value(size, dtype):
     q = torch.randn((1, 4, 1, d), generator=gen(11), device=DEV).to(DT[dtype])
     out = kv4.kv4_decode(q, c.pool, c.table, c.device_lens)
     check_groups(q[0, :, 0], out[0, :, 0], O.rows_value(f32(k)), O.rows_value(f32(v)), d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("heads,d", [((12, 1, 2), 128), ((8, 2, 4), 64), ((16, 4, 4), 128)], ids=str)
+@pytest.mark.parametrize("n", [1021, 20000])
+def test_fp32_is_as_exact_as_binary32(n, heads, d):
+    """Over many positions the weights' relative errors average out like the result, so its relative error, over
+    all heads, is the rms error of a weight. The scores, in powers of two and below 8, are rounded in binary32 about
+    six times on their way: rms 2^-22 / 3^0.5 * 6^0.5 * ln 2 = 2.3e-7. The exponential is within 2^-22, the two terms
+    of a query and of a weight within 2^-23 each: together rms 3.7e-7 at most. 2^-20 is 2.6 times that."""
+    from saga_b200 import kv4
+    hq, hk, hv = heads
+    c = Cache([n], hk, hv, d, 128, "fp32", seed=61)
+    q = torch.randn((1, hq, 1, d), generator=gen(12), device=DEV)
+    out = f64(kv4.kv4_decode(q, c.pool, c.table, c.device_lens))[0, :, 0]
+    ref, _ = O.attention(f64(q[0, :, 0]), c.k[0], c.v[0], np.ones((hk, n), bool), float(np.float32(d ** -0.5)), 0.0)
+    assert np.linalg.norm(out - ref) <= 2.0 ** -20 * np.linalg.norm(ref)
