@@ -135,8 +135,8 @@ __device__ __forceinline__ void mma16_first(float (&c)[4], uint32_t a0, uint32_t
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// log2 of a positive bfloat16 scale, within 0.09 (its bits are a piecewise
-// linear logarithm). It only places the stabilisers.
+// log2 of a positive bfloat16 scale, up to 0.09 below it (its bits are a
+// piecewise linear logarithm). It only places the stabilisers.
 __device__ __forceinline__ float rough_log2(uint32_t bf16_bits) {
   return fmaf(__uint_as_float(0x4b000000u | bf16_bits), 0x1p-7f, -65663.f);
 }
@@ -166,8 +166,8 @@ __device__ __forceinline__ uint32_t centre(uint32_t codes, uint32_t minus) {
 // 4-7; set into the low bits of 1024 they are exact. The tensor cores align the products of a sum by the exponents
 // of their operands, a subnormal's being that of 2^-14: up to ten bits of a product with a code of 2^-24 are lost
 // beside the greatest query or weight. Terms of 22 bits feel that (fp32 errors 3 to 4e-6 with subnormals, 3 to 5e-7
-// without; 4 x 4099 positions 13.0 and 13.4 us), one term of 11 bits does not (fp16 3.0e-4 both ways, and 8 x 32,768
-// positions 29.3 and 29.8 us).
+// without; 4 x 4099 positions 13.0 and 13.4 us), one term of 11 bits does not (fp16 errors are the same both ways, and
+// 8 x 32,768 positions take 29.3 and 29.8 us).
 __device__ __forceinline__ uint32_t whole(uint32_t codes) {
   const uint32_t u = codes | 0x64006400u;
   const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(-1024.f, -1024.f));
@@ -232,7 +232,7 @@ __device__ __forceinline__ long long tiles_per_cta(long long total, int grid) {
 // terms each (fp32 tensors, 22 significant bits). bf16 and fp16 tensors take
 // weights of one fp16 term, which is a choice: its rounding is averaged over the
 // positions, and a second term would double the output's products. Relative rms
-// errors (and those of binary32 arithmetic rounded once): fp16 3.0e-4 (2.1e-4),
+// errors (and those of binary32 arithmetic rounded once): fp16 2.7e-4 (2.1e-4),
 // bf16 1.67e-3 (1.65e-3), fp32 3 to 5e-7 (5 to 15e-7).
 template <int D, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const DecodePlan4 p) {
@@ -242,6 +242,10 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
   // Whether channel rows 0-7 of a product take both codes of a byte, c + 16 c' (rows 8-15 have 16 c' and are
   // taken off at the end): an AND less per code, four bits less of the sums.
   constexpr bool kPairs = !SPLIT;
+  // SPLIT: the stabilisers are whole numbers, so that the factors between them are exact. With one term the
+  // greatest weight is put just below a power of two instead, where it is rounded least (rough_log2 is up to 0.09
+  // below): fp16 errors 2.7e-4 instead of 3.0e-4.
+  constexpr bool kWhole = SPLIT;
   // what a product's one is, in channel rows 0-7 and 8-15
   constexpr float kUnitE = SPLIT ? 0x1p-5f : 0x1p23f, kUnitH = SPLIT ? 0x1p-5f : 0x1p19f;
   constexpr int RP = D + 4;   // pitch of a warp's outputs when the warps meet
@@ -509,7 +513,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
     const uint32_t on_all = sh_on;
 
     f32x2 o[NT][D / 16][2];  // channel rows r8 and r8 + 8, two slots each
-    float mrun[NT], shift[NT][NG];  // the stabilisers, whole numbers
+    float mrun[NT], shift[NT][NG];  // the stabilisers
     f32x2 lsum[NT], zsum[NT][NG];  // over the even and the odd positions
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -677,12 +681,11 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       if (__any_sync(0xffffffffu, raise)) {
         // New ones put the greatest score at or below 0 and the greatest weight, now position by position, at
         // 2^kHead, so that weights far below it are still normal in fp16 (11 significant bits down to 2^-14).
-        // All are whole numbers: the factors between them are exact.
         float down[NT], most[NT][NG];
         quad_max(top_l);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          const float mn = fmaxf(mrun[i], ceilf(top_l[i]));
+          const float mn = fmaxf(mrun[i], kWhole ? ceilf(top_l[i]) : top_l[i]);
           down[i] = mn == kNegInf ? 0.f : mrun[i] - mn;
           mrun[i] = mn;
           const uint8_t* vm = kt + (1 + max(vhl[i], 0)) * TB + META;
@@ -712,7 +715,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
             zsum[i][g] = mul2(zsum[i][g], ff);
             // a scale of 0 (a group that stands for NaN) leaves the shift within what 2^shift can be
             const float to =
-                fmaxf(fminf(fminf(shift[i][g] - down[i], kHead - ceilf(most[i][g])), 126.f), -126.f);
+                fmaxf(fminf(fminf(shift[i][g] - down[i], kHead - (kWhole ? ceilf(most[i][g]) : most[i][g] + 0.09f)),
+                            126.f), -126.f);
             const float fg = ex2(down[i] + (to - shift[i][g]));
             shift[i][g] = to;
             const f32x2 fo = pack2(__shfl_sync(0xffffffffu, fg, 8 * c4), __shfl_sync(0xffffffffu, fg, 8 * c4 + 4));
@@ -746,7 +750,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
             // sum of p (z + 7.5 s): the products below take code - 7.5
             zsum[i][g] = fma2(pp, pack2(kv4_zero(vw[0][g]), kv4_zero(vw[1][g])), zsum[i][g]);
             zsum[i][g] = fma2(middle, w, zsum[i][g]);
-            const float up = exp2_whole(shift[i][g]);
+            const float up = kWhole ? exp2_whole(shift[i][g]) : ex2(shift[i][g]);
             float w0, w1;
             unpack2(mul2(w, pack2(up, up)), w0, w1);
             uint32_t& hi = wb[j >> 1][0][i][g][j & 1];
@@ -859,7 +863,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(const Decode
       for (int g = 0; g < NG; ++g) {
         z0[g] = __shfl_sync(0xffffffffu, lz[g], 8 * c4);
         z1[g] = __shfl_sync(0xffffffffu, lz[g], 8 * c4 + 4);
-        const float u = exp2_whole(-shift[i][g]);
+        const float u = kWhole ? exp2_whole(-shift[i][g]) : ex2(-shift[i][g]);
         u0[g] = __shfl_sync(0xffffffffu, u, 8 * c4);
         u1[g] = __shfl_sync(0xffffffffu, u, 8 * c4 + 4);
       }
