@@ -115,6 +115,19 @@ int check_rows(const SagaKv4Pool* p, int dtype, int64_t T, const void* k, const 
 
 }  // namespace
 
+namespace saga {
+int sm_count() {
+  static thread_local int dev_of = -1, sms = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev != dev_of) {
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    dev_of = dev;
+  }
+  return sms > 0 ? sms : 148;
+}
+}  // namespace saga
+
 extern "C" {
 
 size_t saga_kv4_page_bytes(int32_t D, int32_t page_len) {

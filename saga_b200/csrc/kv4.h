@@ -20,6 +20,8 @@ constexpr int kKv4Tile = 32;  // positions of a tile: its codes and its scales a
 
 __host__ __device__ constexpr int kv4_tile_bytes(int D) { return kKv4Tile * (D / 2 + D / 16); }
 
+int sm_count();  // of the current device
+
 int launch_kv4_write(const SagaKv4Pool& p, int dt, int64_t T, const void* k, int64_t k_st, int64_t k_sh,
                      const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots, int* status, cudaStream_t st);
 int launch_kv4_read(const SagaKv4Pool& p, int dt, int64_t T, const int64_t* slots, void* k, int64_t k_st,

@@ -1029,17 +1029,6 @@ struct DecodeSizes {
   size_t off_o, off_ml, total;
 };
 
-int sm_count() {
-  static thread_local int dev_of = -1, sms = 0;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev != dev_of) {
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    dev_of = dev;
-  }
-  return sms > 0 ? sms : 148;
-}
-
 DecodeSizes decode_sizes(const SagaKv4Args& a) {
   DecodeSizes z;
   const int D = a.pool.D, G = a.Hq / a.pool.Hk, Gv = a.Hq / a.pool.Hv;

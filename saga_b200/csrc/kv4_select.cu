@@ -299,7 +299,8 @@ int launch_kv4_select(const SagaKv4Args& a, cudaStream_t st) {
   if (a.max_pages > a.top) {
     // one page per warp where the SMs hold that many warps, else up to eight
     const int64_t warps = (int64_t)rows * a.max_pages;
-    const int per_warp = (int)std::min<int64_t>(kScorePages, (warps + 16 * 148 - 1) / (16 * 148));
+    const int64_t held = 16ll * sm_count();
+    const int per_warp = (int)std::min<int64_t>(kScorePages, (warps + held - 1) / held);
     const dim3 grid((a.max_pages + 8 * per_warp - 1) / (8 * per_warp), rows);
     auto go = [&](auto* t, auto d) {
       using T = std::remove_pointer_t<decltype(t)>;
