@@ -324,7 +324,12 @@ typedef enum { SAGA_KV4_DECODE = 0, SAGA_KV4_SELECT = 1 } saga_kv4_op;
 SAGA_API size_t saga_kv4_workspace_bytes(const SagaKv4Args* args, int32_t op);
 
 /* Attention of one query position per request over the 4-bit cache. A request
- * without positions gets zeros. */
+ * without positions gets zeros. A value group that stands for NaN makes its 64
+ * channels of its heads NaN and no others; a key row with one makes its heads
+ * NaN. Scores, sums and outputs are binary32; queries and the products of
+ * weights and scales are rounded to 11 significant bits (bf16, fp16) or 22
+ * (fp32). A group's result does not depend on how great the values of other
+ * groups are. Queries have to be below 2^120 in size. */
 SAGA_API int saga_kv4_decode(const SagaKv4Args* args, void* stream);
 
 /* Selects `top` pages per request and key head. The score of a complete page is
@@ -332,8 +337,10 @@ SAGA_API int saga_kv4_decode(const SagaKv4Args* args, void* stream);
  * lo_d), in binary32, summed by halves (d with d + D/2, then d + D/4, ...). The
  * first keep_first and the last keep_last pages of [0, lens[b]) are always
  * kept; of equal scores the lower page is kept; a page with a NaN score is
- * lowest. lo <= hi is assumed. Requests
- * with at most `top` pages keep them all. Needs the pool's bounds. */
+ * lowest. lo <= hi and finite queries are assumed. Requests
+ * with at most `top` pages keep them all. Needs the pool's bounds. `starts` is
+ * not read: pages that lie before a window may be among those chosen (the first
+ * keep_first always are), and decode then leaves their positions out. */
 SAGA_API int saga_kv4_select(const SagaKv4Args* args, void* stream);
 
 /* Block tables and slot maps of one step, from the requests' lengths. Request b
@@ -341,7 +348,10 @@ SAGA_API int saga_kv4_select(const SagaKv4Args* args, void* stream);
  * offsets[b] .. offsets[b + 1] of the step's num_tokens rows. Pages are taken
  * from the front of a ring of free pages, in order of the requests; a request
  * whose pages, table row or token rows do not suffice gets nothing: its tokens
- * get slot -1, its length stays and SAGA_STATUS_OUT_OF_PAGES is set. new_lens[b]
+ * get slot -1, its length stays and SAGA_STATUS_OUT_OF_PAGES is set. The order
+ * is kept where pages are short: after a request that did not get its pages, none
+ * that needs a page gets one in this step (so what must not wait, such as running
+ * requests' single tokens, comes before long prompts). new_lens[b]
  * < 0 finishes request b: its pages go to the ring's end and its length becomes
  * 0. The ring has to have room for every page; a finished request whose pages
  * find none keeps them and its length, and SAGA_STATUS_PAGE_RANGE is set. lens_out and free_state_out may be lens and free_state themselves. */

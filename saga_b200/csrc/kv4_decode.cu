@@ -18,7 +18,8 @@
 // Products: mma.sync m16n8k16 in fp16 with operands built in registers. A code
 // masked out of its word, unshifted, is a subnormal fp16: bits 0-3 are code *
 // 2^-24, bits 4-7 are code * 2^-20, so eight codes become four operand
-// registers with one shift and four ANDs. Feeding tcgen05 instead would put the
+// registers with one shift and four ANDs (for fp32 tensors they are made normal
+// numbers first, see whole()). Feeding tcgen05 instead would put the
 // widened codes through shared memory (4x the bytes of the cache, written and
 // read), which at the HBM rate would already fill its bandwidth.
 //   scores: A = queries (slots x channels), B = codes (channels x positions)
@@ -26,14 +27,15 @@
 //           B = weights (positions x slots): the scores' accumulators have
 //           exactly this layout, so the weights never leave their lane.
 //
-// Measured (with the join): 64 x 65,600 positions, 12 query, 1 key and 4 value
-// heads of 128, 338 us for 1.51 GB, 4.5 TB/s; 8 x 32,768, 12/1/2 heads, 26.6 us
-// for 56.6 MB, 2.1 TB/s. What bounds it is not the memory but the work per code:
+// Measured, per call with the join: 64 x 65,600 positions, 12 query, 1 key and 4
+// value heads of 128, bf16, 361 us for 1.51 GB, 4.2 TB/s (337 us back to back on
+// one cache); 8 x 32,768, 12/1/2 heads, 29.4 us for 56.6 MB, 1.9 TB/s (27.7 us
+// back to back, from L2). What bounds it is not the memory but the work per code:
 // the schedulers issue in 43 % of the cycles and the logical operations take 34 %
-// of theirs, and with 242 registers a thread there are two warps per scheduler to
+// of theirs, and with 254 registers a thread there are two warps per scheduler to
 // cover the products' latency. Twelve warps spill and gain nothing; scores in
 // e4m3, whose instruction is twice as fast, need a further term per query and
-// its registers (31 us instead of 27).
+// its registers (31 us instead of 27, back to back).
 #include <algorithm>
 
 #include "kv4.cuh"

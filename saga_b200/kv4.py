@@ -320,7 +320,7 @@ def kv4_decode(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     Request b attends to its positions [starts[b], lens[b]) (int32 [B]; no
     ``starts`` = 0: a start serves padding on the left or a sliding window).
     ``page_table`` is int32 [B, max_pages]. A request without positions gets
-    zeros. With ``blocks`` and ``counts`` (``kv4_select``) each key head attends
+    zeros; a value group that stands for NaN reaches its own channels alone. With ``blocks`` and ``counts`` (``kv4_select``) each key head attends
     to those pages alone. ``scaling`` defaults to 1/sqrt(D).
     """
     if torch.compiler.is_compiling():
@@ -363,7 +363,9 @@ def kv4_select(query: torch.Tensor, pool: Kv4Pool, page_table: torch.Tensor, len
     Returns ``blocks`` int32 [B, Hk, top], ascending, -1 beyond ``counts`` int32
     [B, Hk]. The first ``keep_first`` and the last ``keep_last`` (>= 1: the last
     page is still filling) pages are always kept; ties go to the lower page;
-    a request with at most ``top`` pages keeps them all.
+    a request with at most ``top`` pages keeps them all. A window's start is not
+    taken: pages before it may be chosen, which ``kv4_decode`` with ``starts``
+    leaves out, so ask for that many more.
     """
     if torch.compiler.is_compiling():
         return torch.ops.saga.kv4_select(*_tensors(pool), query, page_table, lens, top, keep_first, keep_last)
@@ -409,6 +411,8 @@ def page_tables(page_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Te
     of free entries) and are entered in ``page_table`` (int32 [B, max_pages], in
     place). A request that cannot be given all its pages, table entries or rows
     gets nothing: slots -1, its length unchanged, ``STATUS_OUT_OF_PAGES`` set.
+    Pages are granted in order: after a request that did not get its pages, none
+    that needs a page gets one in this step, so running requests come first.
     ``new_lens[b] < 0`` finishes request b: its pages return to the ring's end
     and its length becomes 0 (in a ring without room for them it keeps both, and
     ``STATUS_PAGE_RANGE`` is set).
