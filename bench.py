@@ -25,8 +25,8 @@ Inputs are synthetic (seeded, on the device); 4 rotating KV-cache copies
 --impl reference times the reference's own implementation of the step on the
 host cores (its attention.py, installed unmodified into baseline/_ref by
 baseline/install_reference.sh, with its Triton selection replaced by a torch
-compaction), the whole batch per step, with all torch threads; it falls back to
-the numpy port of its algorithm (oracle/) when the reference is not installed.
+compaction), the whole batch per step, with all torch threads. Where the
+reference is not installed it prints that it is unavailable and times nothing.
 The default line also reports, on the GPU, the reference's own torch + Triton
 step and calibration, this library's calibration step with its roofline, and
 dense GQA decode (this library's kernel and the reference's torch bmm) under
@@ -855,11 +855,12 @@ def main():
             return
         dtn = "fp32" if args.workload == "config1" else "bf16"
         cb = reference_cpu(shape, args.steps, args.warmup, dtn, budget_s=max(60.0, 3.0 * args.steps))
-        if cb is None:  # the reference is not installed: the numpy port of its algorithm
-            cb = cpu_baseline(shape, args.steps, budget_s=max(20.0, 0.5 * args.steps))
+        if cb is None:
+            print(json.dumps({"impl": "reference", "unavailable": "the reference is not installed in baseline/_ref "
+                              "(baseline/install_reference.sh installs it from its sources)"}))
+            return
         line = {"impl": "reference", "metric": metric, "value": cb["value"], "unit": unit, "n_gpus": world,
-                "steps": args.steps, "warmup": args.warmup, "ms_per_step": 1e3 * B / cb["value"] if cb["kind"] == "reference"
-                else 1e3 / cb["value"],
+                "steps": args.steps, "warmup": args.warmup, "ms_per_step": 1e3 * B / cb["value"],
                 "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": dtn,
                 "data": "synthetic", "config": config, "cpu_baseline": cb,
                 "e2e": {"value": cb["value"], "unit": unit, "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}}
